@@ -114,6 +114,10 @@ def lib():
     L.cn_host_csr_lds_rows.restype = None
     L.cn_host_csr_paired_rows.argtypes = [C.c_int]
     L.cn_host_csr_paired_rows.restype = None
+    L.cn_embedding.argtypes = [vp, C.c_int, i64, i64, i64, vp, C.c_int, i64, f32, vp, i64, vp]
+    L.cn_embedding_grad_workspace_bytes.argtypes = [i64, i64, i64]
+    L.cn_embedding_grad_workspace_bytes.restype = sz
+    L.cn_embedding_grad.argtypes = [vp, C.c_int, i64, vp, C.c_int, i64, i64, i64, f32, C.c_int, vp, C.c_int, i64, vp, sz, vp]
     _lib = L
     return L
 
@@ -501,6 +505,100 @@ def rmsprop_update(rms, grad, w, rms_multiplier, learning_rate, precision=None):
         check(lib().cn_rmsprop_update_f32(rms.data_ptr(), grad.data_ptr(), w.data_ptr(), float(rms_multiplier),
                                           float(learning_rate), n, _stream()))
     return rms, w
+
+
+# ---- operators on 32- and 16-bit floats: word tables -----------------------------------------------
+_codes_of_dtype = {}
+
+
+def _dtype_code(t, what, device=None):
+    """The library's number of t's element type; checks that t is a matrix on the GPU with unit column stride."""
+    import torch
+    if not _codes_of_dtype:
+        _codes_of_dtype.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    code = _codes_of_dtype.get(t.dtype) if isinstance(t, torch.Tensor) and t.is_cuda else None
+    if code is None:
+        raise TypeError("%s must be a CUDA/HIP tensor of dtype float32, float16 or bfloat16" % what)
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("%s must be a row-major matrix (unit column stride)" % what)
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError("%s must not have rows that overlap" % what)
+    if device is not None and t.device != device:
+        raise ValueError("%s is on %s, the other operands on %s" % (what, t.device, device))
+    return code
+
+
+def _run(fn, device, *args):
+    """fn(*args, stream) with the tensors' device current and its current stream."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def _tokens(tokens, device):
+    import torch
+    if not (isinstance(tokens, torch.Tensor) and tokens.is_cuda and tokens.dtype in (torch.int32, torch.int64)):
+        raise TypeError("tokens must be a CUDA/HIP tensor of dtype int32 or int64")
+    if not tokens.is_contiguous():
+        raise ValueError("tokens must be contiguous")
+    if tokens.device != device:
+        raise ValueError("tokens are on %s, the other operands on %s" % (tokens.device, device))
+    return 32 if tokens.dtype == torch.int32 else 64
+
+
+def embedding(table, tokens, scale=1.0, out=None):
+    """scale * table[tokens], of shape tokens.shape + (cols,) and the table's type: one row of the table (rows x cols,
+    float32, float16 or bfloat16) per token (int32 or int64), zeros for a token outside the table (padding)."""
+    import torch
+    code = _dtype_code(table, "table")
+    bits = _tokens(tokens, table.device)
+    rows, cols = table.shape
+    count = tokens.numel()
+    if out is None:
+        out = torch.empty(tokens.shape + (cols,), dtype=table.dtype, device=table.device)
+        ldo = cols
+    else:
+        if _dtype_code(out, "out", table.device) != code:
+            raise TypeError("out must be of the table's dtype %s" % table.dtype)
+        if tuple(out.shape) != (count, cols):
+            raise CnError(2, "Matrix size error: out %s, %d tokens of %d columns" % (tuple(out.shape), count, cols))
+        ldo = _ld(out)
+    _run(lib().cn_embedding, table.device, table.data_ptr(), code, rows, cols, _ld(table), tokens.data_ptr(), bits, count, scale,
+         out.data_ptr(), ldo)
+    return out
+
+
+def embedding_grad(dY, tokens, rows, scale=1.0, out=None, out_dtype=None, accumulate=False):
+    """The gradient of `embedding` with respect to its table, rows x cols: row v is scale times the sum of the rows of dY
+    (one per token: tokens.shape + (cols,)) whose token is v, in fp32 and in an order fixed by the tokens.  `out` (or a new
+    matrix of `out_dtype`, dY's type if not given) is float32 or of dY's type.  With `accumulate` the sums are added to
+    `out` and rows that no token names are not touched: scale = -rate makes it the update of the table itself."""
+    import torch
+    if isinstance(dY, torch.Tensor) and dY.dim() != 2 and dY.dim() > 0:
+        dY = dY.view(-1, dY.shape[-1])
+    code = _dtype_code(dY, "dY")
+    bits = _tokens(tokens, dY.device)
+    count, cols = dY.shape
+    if tokens.numel() != count:
+        raise CnError(2, "Matrix size error: %d tokens, dY %s" % (tokens.numel(), tuple(dY.shape)))
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty((rows, cols), dtype=out_dtype or dY.dtype, device=dY.device)
+    out_code = _dtype_code(out, "out", dY.device)
+    if out_code != 0 and out_code != code:
+        raise TypeError("out must be float32 or of dY's dtype %s" % dY.dtype)
+    if tuple(out.shape) != (rows, cols):
+        raise CnError(2, "Matrix size error: out %s, gradient %dx%d" % (tuple(out.shape), rows, cols))
+    L = lib()
+    size = L.cn_embedding_grad_workspace_bytes(count, rows, cols)
+    space = torch.empty(size, dtype=torch.uint8, device=dY.device)
+    _run(L.cn_embedding_grad, dY.device, dY.data_ptr(), code, _ld(dY), tokens.data_ptr(), bits, count, rows, cols, scale,
+         int(accumulate), out.data_ptr(), out_code, _ld(out), space.data_ptr(), size)
+    return out
 
 
 # ---- small kernels around the path (bias, maxout, softmax, ...) ---------------------------------

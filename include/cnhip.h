@@ -47,6 +47,13 @@ enum {
     CN_ERR_ARG = 6         /* any other invalid argument */
 };
 
+/* Element types of the operators that take more than fp32. */
+enum {
+    CN_F32 = 0,
+    CN_F16 = 1,  /* IEEE half precision */
+    CN_BF16 = 2  /* the upper half of an fp32 number */
+};
+
 /* Human-readable name of a status code. */
 const char *cn_status_string(cn_status s);
 /* Text of the most recent failure on the calling thread ("" if none). */
@@ -288,6 +295,32 @@ cn_status cn_csr_to_dense_f32(int64_t R, int64_t C, const int32_t *row_ptr_devic
 cn_status cn_csr_transpose(int64_t R, int64_t C, int64_t nnz, const int32_t *row_ptr_device,
                            const int32_t *col_idx_device, const float *vals_device, int32_t *t_row_ptr_device,
                            int32_t *t_col_idx_device, float *t_vals_device, int32_t *scratch_device, void *stream);
+
+/* ---- models that read words ----------------------------------------------------------------------
+ * A table of one row per word stands in for a first layer on one-hot inputs.  The reference gathers the windows of
+ * its language model from such a table and scatters their gradient back with atomics (kConstructVocabMatrix,
+ * kUpdateVocabWithGradient, source/clusterKernels.cu:1497-1712; launchers source/basicOps.cu:1352-1430).
+ * Tokens are int32 (token_bits 32) or int64 (64) row numbers; a token outside [0, rows) names no row (padding). */
+
+/* out[t][:] = scale * table[tokens[t]][:], rounded once to the table's type; zeros where the token names no row.
+ * table: rows x cols of `dtype` (CN_F32, CN_F16, CN_BF16), leading dimension ld; out: count x cols, ldo. */
+cn_status cn_embedding(const void *table_device, int dtype, int64_t rows, int64_t cols, int64_t ld,
+                       const void *tokens_device, int token_bits, int64_t count, float scale, void *out_device,
+                       int64_t ldo, void *stream);
+
+/* The gradient of cn_embedding with respect to its table, dE[v][:] = scale * sum of dY[t][:] over the t with
+ * tokens[t] == v, summed in fp32 in an order that depends on the tokens alone (the same bits every time).
+ * accumulate == 0: all rows x cols of dE are written, zeros where no token names the row;
+ * accumulate != 0: the sums are added to dE, and rows that no token names are left as they are: with scale = -rate it is
+ * the update of the reference's kUpdateVocabWithGradient.
+ * dY: count x cols of dy_dtype; dE: rows x cols, fp32 or of dy_dtype (then added up in fp32 and rounded once).
+ * `workspace`: cn_embedding_grad_workspace_bytes(count, rows, cols) bytes of device memory, aligned to 256, the caller's
+ * until the call has run; calls with workspaces of their own may overlap.  dE must not overlap dY. */
+size_t cn_embedding_grad_workspace_bytes(int64_t count, int64_t rows, int64_t cols);
+cn_status cn_embedding_grad(const void *dY_device, int dy_dtype, int64_t ldy, const void *tokens_device,
+                            int token_bits, int64_t count, int64_t rows, int64_t cols, float scale, int accumulate,
+                            void *dE_device, int de_dtype, int64_t lde, void *workspace_device,
+                            size_t workspace_bytes, void *stream);
 
 /* ---- small kernels used around the path by its callers (row-major, flat where no shape is given).
  * They are not on the measured hot path; each names the reference routine it stands in for. */

@@ -1,0 +1,67 @@
+"""Calls that the word-table, update and 4-bit operators refuse, checked without a GPU: the C entry points look at their
+arguments before they need a device (the addresses here are never read), the binding before it calls them."""
+import pytest
+
+import clusternet_amd as cn
+
+SHAPE, NULL, ARG, WORKSPACE, NO_DEVICE = 2, 1, 6, 5, 3
+AT = 4096  # an address that no call gets as far as reading
+
+
+def _refused(status, want):
+    assert status == want, (status, cn.lib().cn_last_error())
+    assert cn.lib().cn_last_error() != b""
+
+
+def test_embedding_refuses():
+    f = cn.lib().cn_embedding
+    _refused(f(AT, 3, 4, 4, 4, AT, 32, 4, 1.0, AT, 4, None), ARG)        # no such type
+    _refused(f(AT, 0, -1, 4, 4, AT, 32, 4, 1.0, AT, 4, None), SHAPE)
+    _refused(f(AT, 0, 4, 4, 3, AT, 32, 4, 1.0, AT, 4, None), SHAPE)      # leading dimensions
+    _refused(f(AT, 0, 4, 4, 4, AT, 32, 4, 1.0, AT, 3, None), SHAPE)
+    _refused(f(AT, 0, 4, 4, 4, AT, 16, 4, 1.0, AT, 4, None), ARG)        # 16-bit tokens
+    _refused(f(AT, 0, 4, 4, 4, AT, 32, -4, 1.0, AT, 4, None), SHAPE)
+    _refused(f(AT, 0, 4, 4, 4, AT, 32, 2 ** 31, 1.0, AT, 4, None), SHAPE)
+    _refused(f(AT, 0, 2 ** 31, 4, 4, AT, 32, 4, 1.0, AT, 4, None), SHAPE)
+    _refused(f(None, 0, 4, 4, 4, AT, 32, 4, 1.0, AT, 4, None), NULL)
+    _refused(f(AT, 0, 4, 4, 4, None, 32, 4, 1.0, AT, 4, None), NULL)
+    _refused(f(AT, 0, 4, 4, 4, AT, 32, 4, 1.0, None, 4, None), NULL)
+    assert f(None, 0, 0, 4, 4, None, 32, 0, 1.0, None, 4, None) == 0     # no tokens: nothing to do
+
+
+def test_embedding_grad_refuses():
+    L = cn.lib()
+    f, need = L.cn_embedding_grad, L.cn_embedding_grad_workspace_bytes
+    size = need(100, 50, 8)
+    assert size > 100 * 16 and need(0, 50, 8) == 0 and need(100, 50, 0) == 0 and need(-1, 50, 8) == 0
+    ok = [AT, 0, 8, AT, 32, 100, 50, 8, 1.0, 0, AT, 0, 8, AT, size, None]
+
+    def call(**change):
+        a = list(ok)
+        for k, v in change.items():
+            a[int(k[1:])] = v
+        return f(*a)
+    _refused(call(_1=7), ARG)
+    _refused(call(_1=1, _11=2), ARG)          # fp16 errors, bf16 gradient
+    _refused(call(_11=1), ARG)                # fp32 errors, fp16 gradient
+    _refused(call(_2=7), SHAPE)
+    _refused(call(_12=7), SHAPE)
+    _refused(call(_4=8), ARG)
+    _refused(call(_5=-1), SHAPE)
+    _refused(call(_6=-1), SHAPE)
+    _refused(call(_7=-1), SHAPE)
+    _refused(call(_6=2 ** 31), SHAPE)
+    for place in ("_0", "_3", "_10", "_13"):
+        _refused(call(**{place: None}), NULL)
+    _refused(call(_14=size - 1), WORKSPACE)
+    _refused(call(_13=AT + 16), ARG)          # alignment of the workspace
+    assert call(_5=0, _9=1, _0=None, _3=None, _13=None, _14=0) == 0
+
+
+def test_binding_refuses_tensors_of_the_host():
+    torch = pytest.importorskip("torch")
+    table, tokens = torch.zeros(4, 4), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(TypeError):
+        cn.embedding(table, tokens)
+    with pytest.raises(TypeError):
+        cn.embedding_grad(table, tokens, 4)
