@@ -4,8 +4,10 @@ ClusterNet / Matrix facade over it; this package is the thin Python host binding
 tests and the benchmark.  PyTorch appears only as the owner of device memory and streams.
 """
 from ._lib import (CnError, absmax, absmax_compression_8bit, compression_8bit, compression_8bit_axpy, decompression_8bit, decompression_8bit_axpy, dot, dotT,
-                   embedding, embedding_grad, Tdot, gemm, gemm_w8, init, lib, lib_path, num_compute_units, rmsprop_update, table)
+                   embedding, embedding_grad, Tdot, gemm, gemm_w8, init, lib, lib_path,
+                   muon_update, num_compute_units, orthogonalize, rmsprop_update, table)
 
 __all__ = ["CnError", "absmax", "absmax_compression_8bit", "compression_8bit", "compression_8bit_axpy", "decompression_8bit", "decompression_8bit_axpy", "dot",
-           "dotT", "embedding", "embedding_grad", "Tdot", "gemm", "gemm_w8", "init", "lib", "lib_path", "num_compute_units", "rmsprop_update",
+           "dotT", "embedding", "embedding_grad", "Tdot", "gemm", "gemm_w8", "init", "lib", "lib_path", "muon_update", "num_compute_units",
+           "orthogonalize", "rmsprop_update",
            "table"]

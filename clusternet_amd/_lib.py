@@ -118,6 +118,10 @@ def lib():
     L.cn_embedding_grad_workspace_bytes.argtypes = [i64, i64, i64]
     L.cn_embedding_grad_workspace_bytes.restype = sz
     L.cn_embedding_grad.argtypes = [vp, C.c_int, i64, vp, C.c_int, i64, i64, i64, f32, C.c_int, vp, C.c_int, i64, vp, sz, vp]
+    L.cn_orthogonalize_workspace_bytes.argtypes = [i64, i64]
+    L.cn_orthogonalize_workspace_bytes.restype = sz
+    L.cn_orthogonalize.argtypes = [vp, C.c_int, i64, i64, i64, C.c_int, vp, C.c_int, i64, vp, sz, vp]
+    L.cn_muon_update.argtypes = [vp, i64, vp, C.c_int, i64, vp, i64, i64, i64, f32, C.c_int, f32, f32, C.c_int, vp, sz, vp]
     _lib = L
     return L
 
@@ -507,7 +511,7 @@ def rmsprop_update(rms, grad, w, rms_multiplier, learning_rate, precision=None):
     return rms, w
 
 
-# ---- operators on 32- and 16-bit floats: word tables -----------------------------------------------
+# ---- operators on 32- and 16-bit floats: word tables, updates of whole matrices -----------------------------------------------
 _codes_of_dtype = {}
 
 
@@ -599,6 +603,45 @@ def embedding_grad(dY, tokens, rows, scale=1.0, out=None, out_dtype=None, accumu
     _run(L.cn_embedding_grad, dY.device, dY.data_ptr(), code, _ld(dY), tokens.data_ptr(), bits, count, rows, cols, scale,
          int(accumulate), out.data_ptr(), out_code, _ld(out), space.data_ptr(), size)
     return out
+
+
+def orthogonalize(G, steps=5, out=None):
+    """G with its singular values moved towards one by `steps` Newton-Schulz products, to fp32 accuracy; `out` (G's type if
+    not given; float32, float16 or bfloat16) may be G itself."""
+    import torch
+    code = _dtype_code(G, "G")
+    if out is None:
+        out = torch.empty(G.shape, dtype=G.dtype, device=G.device)
+    out_code = _dtype_code(out, "out", G.device)
+    if out.shape != G.shape:
+        raise CnError(2, "Matrix size error: G %s, out %s" % (tuple(G.shape), tuple(out.shape)))
+    rows, cols = G.shape
+    L = lib()
+    size = L.cn_orthogonalize_workspace_bytes(rows, cols)
+    space = torch.empty(size, dtype=torch.uint8, device=G.device)
+    _run(L.cn_orthogonalize, G.device, G.data_ptr(), code, rows, cols, _ld(G), int(steps), out.data_ptr(), out_code, _ld(out),
+         space.data_ptr(), size)
+    return out
+
+
+def muon_update(momentum, grad, w, momentum_factor, learning_rate, nesterov=True, weight_decay=0.0, steps=5):
+    """Weight update along the orthogonalised momentum (the Muon rule), in place on momentum and w (float32); `grad` is
+    float32, float16 or bfloat16."""
+    import torch
+    _need(momentum, torch.float32, "momentum")
+    _need(w, torch.float32, "w")
+    code = _dtype_code(grad, "grad")
+    if _dtype_code(momentum, "momentum", grad.device) or _dtype_code(w, "w", grad.device):
+        raise TypeError("momentum and w must be float32")
+    if momentum.shape != w.shape or grad.shape != w.shape:
+        raise CnError(2, "Matrix size error: momentum %s, grad %s, w %s" % (tuple(momentum.shape), tuple(grad.shape), tuple(w.shape)))
+    rows, cols = w.shape
+    L = lib()
+    size = L.cn_orthogonalize_workspace_bytes(rows, cols)
+    space = torch.empty(size, dtype=torch.uint8, device=w.device)
+    _run(L.cn_muon_update, w.device, momentum.data_ptr(), _ld(momentum), grad.data_ptr(), code, _ld(grad), w.data_ptr(), _ld(w),
+         rows, cols, momentum_factor, int(nesterov), learning_rate, weight_decay, int(steps), space.data_ptr(), size)
+    return momentum, w
 
 
 # ---- small kernels around the path (bias, maxout, softmax, ...) ---------------------------------

@@ -296,6 +296,33 @@ cn_status cn_csr_transpose(int64_t R, int64_t C, int64_t nnz, const int32_t *row
                            const int32_t *col_idx_device, const float *vals_device, int32_t *t_row_ptr_device,
                            int32_t *t_col_idx_device, float *t_vals_device, int32_t *scratch_device, void *stream);
 
+/* ---- updates of whole matrices ------------------------------------------------------------------
+ * Orthogonalised updates: what RMSprop does element by element, for the singular values of a weight matrix's
+ * gradient.  Both take a workspace of cn_orthogonalize_workspace_bytes(rows, cols) bytes of device memory (aligned to
+ * 256, the caller's until the call has run; a few times the matrix); calls with workspaces of their own may overlap.
+ * At most 2^17 rows and columns, 1 to 100 steps.  The same bits every time. */
+
+/* out = the gradient with its singular values moved towards one: X = G / (|G|_F + 1e-7), transposed if rows > cols, then
+ * `steps` times A = X X^T, X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X (five steps bring singular values from 0.002 to 1 of
+ * the largest to between about 0.7 and 1.2).  All of it to fp32 accuracy whatever the types; the result is rounded
+ * once.  G and out are rows x cols, CN_F32, CN_F16 or CN_BF16 each; out may be G.  A zero G gives zeros, one that is
+ * not finite NaNs. */
+size_t cn_orthogonalize_workspace_bytes(int64_t rows, int64_t cols);
+cn_status cn_orthogonalize(const void *G_device, int dtype, int64_t rows, int64_t cols, int64_t ldg, int steps,
+                           void *out_device, int out_dtype, int64_t ldo, void *workspace_device,
+                           size_t workspace_bytes, void *stream);
+
+/* The weight update that moves along it (the Muon rule):
+ *   momentum = momentum_factor * momentum + grad
+ *   u        = nesterov ? grad + momentum_factor * momentum : momentum
+ *   w        = (1 - learning_rate * weight_decay) * w - learning_rate * orthogonalize(u)
+ * momentum and w fp32, the gradient of grad_dtype; every operation rounded to fp32.  A factor for the shape
+ * (such as sqrt(max(1, rows / cols))) is the caller's, in the rate. */
+cn_status cn_muon_update(float *momentum_device, int64_t ldm, const void *grad_device, int grad_dtype, int64_t ldg,
+                         float *w_device, int64_t ldw, int64_t rows, int64_t cols, float momentum_factor,
+                         int nesterov, float learning_rate, float weight_decay, int steps, void *workspace_device,
+                         size_t workspace_bytes, void *stream);
+
 /* ---- models that read words ----------------------------------------------------------------------
  * A table of one row per word stands in for a first layer on one-hot inputs.  The reference gathers the windows of
  * its language model from such a table and scatters their gradient back with atomics (kConstructVocabMatrix,

@@ -65,3 +65,52 @@ def test_binding_refuses_tensors_of_the_host():
         cn.embedding(table, tokens)
     with pytest.raises(TypeError):
         cn.embedding_grad(table, tokens, 4)
+
+
+def test_orthogonalize_refuses():
+    L = cn.lib()
+    need = L.cn_orthogonalize_workspace_bytes
+    size = need(10, 20)
+    assert size > 0 and need(20, 10) == size and need(0, 4) == 0 and need(4, 0) == 0 and need(-1, 4) == 0 and need(2 ** 17 + 1, 4) == 0
+    ok = [AT, 0, 10, 20, 20, 5, AT, 0, 20, AT, size, None]
+
+    def call(**change):
+        a = list(ok)
+        for k, v in change.items():
+            a[int(k[1:])] = v
+        return L.cn_orthogonalize(*a)
+    _refused(call(_1=3), ARG)
+    _refused(call(_7=-1), ARG)
+    _refused(call(_2=-1), SHAPE)
+    _refused(call(_3=-1), SHAPE)
+    _refused(call(_2=2 ** 17 + 1), SHAPE)
+    _refused(call(_4=19), SHAPE)
+    _refused(call(_8=19), SHAPE)
+    _refused(call(_5=0), ARG)
+    _refused(call(_5=101), ARG)
+    for place in ("_0", "_6", "_9"):
+        _refused(call(**{place: None}), NULL)
+    _refused(call(_10=size - 1), WORKSPACE)
+    _refused(call(_9=AT + 128), ARG)
+    assert call(_2=0, _0=None, _6=None, _9=None) == 0
+
+
+def test_muon_update_refuses():
+    L = cn.lib()
+    size = L.cn_orthogonalize_workspace_bytes(10, 20)
+    ok = [AT, 20, AT, 0, 20, AT, 20, 10, 20, 0.9, 1, 0.1, 0.0, 5, AT, size, None]
+
+    def call(**change):
+        a = list(ok)
+        for k, v in change.items():
+            a[int(k[1:])] = v
+        return L.cn_muon_update(*a)
+    _refused(call(_3=5), ARG)
+    for place in ("_1", "_4", "_6"):
+        _refused(call(**{place: 19}), SHAPE)
+    _refused(call(_7=-1), SHAPE)
+    _refused(call(_13=0), ARG)
+    for place in ("_0", "_2", "_5", "_14"):
+        _refused(call(**{place: None}), NULL)
+    _refused(call(_15=size - 1), WORKSPACE)
+    assert call(_8=0, _0=None, _2=None, _5=None, _14=None) == 0
