@@ -122,6 +122,11 @@ def lib():
     L.cn_orthogonalize_workspace_bytes.restype = sz
     L.cn_orthogonalize.argtypes = [vp, C.c_int, i64, i64, i64, C.c_int, vp, C.c_int, i64, vp, sz, vp]
     L.cn_muon_update.argtypes = [vp, i64, vp, C.c_int, i64, vp, i64, i64, i64, f32, C.c_int, f32, f32, C.c_int, vp, sz, vp]
+    L.cn_w4_code_words.argtypes = [i64, i64]
+    L.cn_w4_code_words.restype = sz
+    L.cn_quantize_4bit.argtypes = [vp, C.c_int, i64, i64, i64, C.c_int, vp, vp, vp, vp]
+    L.cn_dequantize_4bit.argtypes = [vp, vp, vp, i64, i64, C.c_int, vp, C.c_int, i64, vp]
+    L.cn_gemm_w4.argtypes = [i64, i64, i64, vp, C.c_int, i64, vp, vp, vp, C.c_int, vp, i64, vp]
     _lib = L
     return L
 
@@ -511,7 +516,7 @@ def rmsprop_update(rms, grad, w, rms_multiplier, learning_rate, precision=None):
     return rms, w
 
 
-# ---- operators on 32- and 16-bit floats: word tables, updates of whole matrices -----------------------------------------------
+# ---- operators on 32- and 16-bit floats: word tables, updates of whole matrices, 4-bit weights -----------------------------------------------
 _codes_of_dtype = {}
 
 
@@ -642,6 +647,78 @@ def muon_update(momentum, grad, w, momentum_factor, learning_rate, nesterov=True
     _run(L.cn_muon_update, w.device, momentum.data_ptr(), _ld(momentum), grad.data_ptr(), code, _ld(grad), w.data_ptr(), _ld(w),
          rows, cols, momentum_factor, int(nesterov), learning_rate, weight_decay, int(steps), space.data_ptr(), size)
     return momentum, w
+
+
+class W4:
+    """Weights inner x outer in 4 bits, (q - z) * s: `codes` (int32, [ceil(outer / 16)][ceil(inner / 128)][64][4]; the order is in
+    cnhip.h), `scales` (float32) and `zeros` (uint8, or None: 8 everywhere) [ceil(inner / group)][outer]."""
+
+    def __init__(self, codes, scales, zeros, inner, outer, group):
+        import torch
+        groups = -(-inner // group) if group > 0 else 0
+        tensors = ((codes, torch.int32, "codes", (-(-outer // 16), -(-inner // 128), 64, 4)),
+                   (scales, torch.float32, "scales", (groups, outer)),
+                   (zeros, torch.uint8, "zeros", (groups, outer)))
+        for t, dtype, what, shape in tensors:
+            if t is None and what == "zeros":
+                continue
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype):
+                raise TypeError("%s must be a CUDA/HIP tensor of dtype %s" % (what, dtype))
+            if t.shape != shape or not t.is_contiguous():
+                raise ValueError("%s must be a contiguous tensor of shape %s (got %s)" % (what, shape, tuple(t.shape)))
+            if t.device != codes.device:
+                raise ValueError("%s is on %s, the codes on %s" % (what, t.device, codes.device))
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+        self.inner, self.outer, self.group = inner, outer, group
+
+
+def quantize_4bit(W, group=128, zero_points=False):
+    """W (inner x outer; float32, float16 or bfloat16) in 4 bits with a scale, and with `zero_points` a zero point, per group of
+    32, 64 or 128 rows of a column: a W4."""
+    import torch
+    code = _dtype_code(W, "W")
+    K, N = W.shape
+    if group not in (32, 64, 128):
+        raise ValueError("groups of %d rows (32, 64 or 128)" % group)
+    groups = -(-K // group)
+    codes = torch.empty((-(-N // 16), -(-K // 128), 64, 4), dtype=torch.int32, device=W.device)
+    scales = torch.empty((groups, N), dtype=torch.float32, device=W.device)
+    zeros = torch.empty((groups, N), dtype=torch.uint8, device=W.device) if zero_points else None
+    _run(lib().cn_quantize_4bit, W.device, W.data_ptr(), code, K, N, _ld(W), group, codes.data_ptr(), scales.data_ptr(),
+         None if zeros is None else zeros.data_ptr())
+    return W4(codes, scales, zeros, K, N, group)
+
+
+def dequantize_4bit(W, dtype=None, out=None):
+    """The weights that a W4 stands for, inner x outer (float32 unless `dtype` or `out` says otherwise)."""
+    import torch
+    if out is None:
+        out = torch.empty((W.inner, W.outer), dtype=dtype or torch.float32, device=W.codes.device)
+    code = _dtype_code(out, "out", W.codes.device)
+    if tuple(out.shape) != (W.inner, W.outer):
+        raise CnError(2, "Matrix size error: out %s, weights %dx%d" % (tuple(out.shape), W.inner, W.outer))
+    _run(lib().cn_dequantize_4bit, out.device, W.codes.data_ptr(), W.scales.data_ptr(), None if W.zeros is None else W.zeros.data_ptr(),
+         W.inner, W.outer, W.group, out.data_ptr(), code, _ld(out))
+    return out
+
+
+def gemm_w4(A, W, out=None):
+    """out = A W with W a W4 and A (a row per token) float32, float16 or bfloat16; out is of A's type."""
+    import torch
+    code = _dtype_code(A, "A")
+    M, K = A.shape
+    device = A.device
+    if W.codes.device != device:
+        raise ValueError("W is on %s, A on %s" % (W.codes.device, device))
+    if out is None:
+        out = torch.empty((M, W.outer), dtype=A.dtype, device=device)
+    elif _dtype_code(out, "out", device) != code:
+        raise TypeError("out must be of A's dtype %s" % A.dtype)
+    if K != W.inner or out.shape[0] != M or out.shape[1] != W.outer:
+        raise CnError(2, "Matrix size error: A %s, W %dx%d, out %s" % (tuple(A.shape), W.inner, W.outer, tuple(out.shape)))
+    _run(lib().cn_gemm_w4, device, M, W.outer, K, A.data_ptr(), code, _ld(A), W.codes.data_ptr(), W.scales.data_ptr(),
+         None if W.zeros is None else W.zeros.data_ptr(), W.group, out.data_ptr(), _ld(out))
+    return out
 
 
 # ---- small kernels around the path (bias, maxout, softmax, ...) ---------------------------------

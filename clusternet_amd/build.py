@@ -25,7 +25,7 @@ HIP_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-ffp-contr
              "-Wno-inline-asm"]
 SOURCES = ["cn_runtime.cpp", "cn_encode_lut.cpp", "cn_gemm_plan.cpp", "cn_codec.hip", "cn_gemm.hip", "cn_gemm_w8_rows.hip", "cn_gemm_small.hip", "cn_gemm_c8c8.hip",
            "cn_layers.hip", "cn_update.hip", "cn_sparse.hip", "cn_embedding.hip",
-           "cn_orthogonalize.hip"]
+           "cn_orthogonalize.hip", "cn_w4.hip"]
 
 
 def hipcc():

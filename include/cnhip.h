@@ -296,6 +296,32 @@ cn_status cn_csr_transpose(int64_t R, int64_t C, int64_t nnz, const int32_t *row
                            const int32_t *col_idx_device, const float *vals_device, int32_t *t_row_ptr_device,
                            int32_t *t_col_idx_device, float *t_vals_device, int32_t *scratch_device, void *stream);
 
+/* ---- weights in 4 bits ---------------------------------------------------------------------------
+ * W (K x N) = (q - z) * s with q in 0 .. 15, a scale s (fp32) and a zero point z per group of 32, 64 or 128 rows of a
+ * column.  scales and zeros are [ceil(K / group)][N]; zeros (bytes 0 .. 15) may be NULL: 8 everywhere.
+ * codes: cn_w4_code_words(K, N) int32 words [ceil(N / 16)][ceil(K / 128)][64][4], aligned to 16 bytes: nibble i (bits 4 i
+ * and up) of word t of entry 16 h + c holds row 128 b + 32 t + 8 h + i of column 16 a + c; rows and columns past the
+ * matrix hold 0. */
+size_t cn_w4_code_words(int64_t K, int64_t N);
+
+/* W (K x N of `dtype`, leading dimension ldw) to that form.  Without zeros: s = max|w| / 7, q = round(w / s) + 8; with
+ * zeros, from the range of the group and 0: s = (max - min) / 15, z = round(-min / s), q = round(w / s) + z, kept in 0 .. 15.
+ * s is rounded to fp32 once, quotients are rounded to the nearest whole number exactly (halves to even).  A group
+ * with a value that is not finite gets the scale NaN.  The reference has no such format; its codec is the 8-bit one. */
+cn_status cn_quantize_4bit(const void *W_device, int dtype, int64_t K, int64_t N, int64_t ldw, int group,
+                           int32_t *codes_device, float *scales_device, uint8_t *zeros_device, void *stream);
+/* out (K x N of `dtype`) = (q - z) * s, the product rounded to fp32 and once more to 16 bits. */
+cn_status cn_dequantize_4bit(const int32_t *codes_device, const float *scales_device, const uint8_t *zeros_device,
+                             int64_t K, int64_t N, int group, void *out_device, int dtype, int64_t ldo, void *stream);
+
+/* out (M x N) = A (M x K) W with W in that form; A and out of `dtype`.  Products are exact, sums and scales fp32, a
+ * 16-bit result is rounded once.  Made for answers (a row per token, up to a few dozen); any M is right, but from a few
+ * hundred rows on decoded weights are faster.  The same bits every time; needs no workspace.  A row of A with a number
+ * that is not finite gives NaNs.  The 8-bit relative is cn_gemm_f32_w8. */
+cn_status cn_gemm_w4(int64_t M, int64_t N, int64_t K, const void *A_device, int dtype, int64_t lda,
+                     const int32_t *codes_device, const float *scales_device, const uint8_t *zeros_device, int group,
+                     void *out_device, int64_t ldo, void *stream);
+
 /* ---- updates of whole matrices ------------------------------------------------------------------
  * Orthogonalised updates: what RMSprop does element by element, for the singular values of a weight matrix's
  * gradient.  Both take a workspace of cn_orthogonalize_workspace_bytes(rows, cols) bytes of device memory (aligned to

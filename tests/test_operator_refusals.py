@@ -114,3 +114,61 @@ def test_muon_update_refuses():
         _refused(call(**{place: None}), NULL)
     _refused(call(_15=size - 1), WORKSPACE)
     assert call(_8=0, _0=None, _2=None, _5=None, _14=None) == 0
+
+
+def test_w4_refuses():
+    L = cn.lib()
+    assert L.cn_w4_code_words(128, 16) == 256 and L.cn_w4_code_words(129, 17) == 4 * 256
+    assert L.cn_w4_code_words(0, 16) == 0 and L.cn_w4_code_words(16, -1) == 0
+
+    def caller(f, ok):
+        def call(**change):
+            a = list(ok)
+            for k, v in change.items():
+                a[int(k[1:])] = v
+            return f(*a)
+        return call
+    q = caller(L.cn_quantize_4bit, [AT, 0, 64, 32, 32, 32, AT, AT, AT, None])
+    _refused(q(_1=9), ARG)
+    _refused(q(_2=-1), SHAPE)
+    _refused(q(_3=-1), SHAPE)
+    _refused(q(_4=31), SHAPE)
+    for group in (0, -32, 16, 48, 256):
+        _refused(q(_5=group), ARG)
+    for place in ("_0", "_6", "_7"):
+        _refused(q(**{place: None}), NULL)
+    _refused(q(_6=AT + 4), ARG)
+    _refused(q(_2=2 ** 31), SHAPE)
+    assert q(_2=0, _0=None, _6=None, _7=None) == 0
+    d = caller(L.cn_dequantize_4bit, [AT, AT, AT, 64, 32, 32, AT, 0, 32, None])
+    _refused(d(_7=9), ARG)
+    _refused(d(_5=33), ARG)
+    _refused(d(_8=31), SHAPE)
+    for place in ("_0", "_1", "_6"):
+        _refused(d(**{place: None}), NULL)
+    _refused(d(_0=AT + 8), ARG)
+    g = caller(L.cn_gemm_w4, [4, 32, 64, AT, 0, 64, AT, AT, AT, 32, AT, 32, None])
+    _refused(g(_4=9), ARG)
+    _refused(g(_0=-1), SHAPE)
+    _refused(g(_1=-1), SHAPE)
+    _refused(g(_2=-1), SHAPE)
+    _refused(g(_5=63), SHAPE)
+    _refused(g(_11=31), SHAPE)
+    _refused(g(_9=96), ARG)
+    _refused(g(_0=2 ** 20 + 1), SHAPE)
+    for place in ("_3", "_6", "_7", "_10"):
+        _refused(g(**{place: None}), NULL)
+    _refused(g(_6=AT + 8), ARG)
+    assert g(_0=0, _3=None, _6=None, _7=None, _10=None) == 0
+
+
+def test_w4_binding_refuses():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(TypeError):
+        cn.quantize_4bit(torch.zeros(32, 16))
+    with pytest.raises(TypeError):
+        cn.W4(torch.zeros(1, 1, 64, 4, dtype=torch.int32), torch.zeros(1, 16), None, 32, 16, 32)
+    with pytest.raises(TypeError):
+        cn.orthogonalize(torch.zeros(3, 3))
+    with pytest.raises(TypeError):
+        cn.muon_update(torch.zeros(3, 3), torch.zeros(3, 3), torch.zeros(3, 3), 0.9, 0.1)
