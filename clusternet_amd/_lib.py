@@ -522,29 +522,52 @@ _codes_of_dtype = {}
 
 def _dtype_code(t, what, device=None):
     """The library's number of t's element type; checks that t is a matrix on the GPU with unit column stride."""
-    import torch
     if not _codes_of_dtype:
+        import torch
         _codes_of_dtype.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-    code = _codes_of_dtype.get(t.dtype) if isinstance(t, torch.Tensor) and t.is_cuda else None
-    if code is None:
+    code = _codes_of_dtype.get(getattr(t, "dtype", None))
+    if code is None or not getattr(t, "is_cuda", False):
         raise TypeError("%s must be a CUDA/HIP tensor of dtype float32, float16 or bfloat16" % what)
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError("%s must be a row-major matrix (unit column stride)" % what)
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError("%s must not have rows that overlap" % what)
+    if t.dim() != 2:
+        raise ValueError("%s must be a matrix" % what)
+    if not t.is_contiguous():
+        rows, cols = t.shape
+        if cols > 1 and t.stride(1) != 1:
+            raise ValueError("%s must be row-major (unit column stride)" % what)
+        if rows > 1 and t.stride(0) < cols:
+            raise ValueError("%s must not have rows that overlap" % what)
     if device is not None and t.device != device:
         raise ValueError("%s is on %s, the other operands on %s" % (what, t.device, device))
     return code
 
 
+_current = None
+
+
+def _device_and_stream():
+    """(current device, its current stream as an address) without the objects of the public calls, which cost 2 us of a small
+    call's 10; the public calls where this PyTorch lacks them."""
+    import torch
+    try:
+        return torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    except AttributeError:
+        return torch.cuda.current_device, lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
 def _run(fn, device, *args):
     """fn(*args, stream) with the tensors' device current and its current stream."""
-    import torch
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    global _current
+    if _current is None:
+        _current = _device_and_stream()
+    index = device.index
+    if index == _current[0]():
+        status = fn(*args, _current[1](index))
     else:
+        import torch
         with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+            status = fn(*args, _current[1](index))
+    if status:
+        check(status)
 
 
 def _tokens(tokens, device):
@@ -611,8 +634,8 @@ def embedding_grad(dY, tokens, rows, scale=1.0, out=None, out_dtype=None, accumu
 
 
 def orthogonalize(G, steps=5, out=None):
-    """G with its singular values moved towards one by `steps` Newton-Schulz products, to fp32 accuracy; `out` (G's type if
-    not given; float32, float16 or bfloat16) may be G itself."""
+    """G with its singular values moved towards one by `steps` Newton-Schulz steps, to the accuracy of fp32 products (1e-3 where
+    the result is bfloat16); `out` (G's type if not given; float32, float16 or bfloat16) may be G itself."""
     import torch
     code = _dtype_code(G, "G")
     if out is None:

@@ -9,23 +9,29 @@
 //
 // The products are what this costs: 3 m^2 n + m^3 multiply-adds per step after the symmetry of A and A A (only tiles on and
 // above the diagonal are computed).  In fp32 the matrix cores give 157 TFLOP/s; here each operand is kept as two fp16
-// numbers, x 2^14 = hi + lo, and a product is the three fp16 products hi hi + hi lo + lo hi in fp32 accumulators, which
-// runs at up to a third of the fp16 rate (2.5 PFLOP/s).  What is left out, lo lo, and the rounding of lo are 2^-22 of the
-// product, so the result is as far from the exact one as plain fp32 products leave it (measured on the CPU for
-// Gaussian, power-law and nearly rank-8 spectra: within 5 % of fp32's error in every case).  The factor 2^14 keeps
-// entries of all four matrices below 65504 (|X| <= 1.21, |A| <= 1.46, |P| <= 2.81) and lo above the smallest
-// fp16 number for entries down to 2^-13 of the largest.  a X stays outside the product, with X read back as hi + lo:
-// folding a into P's diagonal costs a factor of three in accuracy for nearly low-rank gradients.
+// numbers, x 2^14 = hi + lo, and a product is the three fp16 products hi hi + hi lo + lo hi in fp32 accumulators.  What
+// is left out, lo lo, and the rounding of lo are 2^-22 of the product, so the result is as far from the exact one as plain
+// fp32 products leave it (emulated on the CPU for Gaussian, power-law and nearly rank-8 spectra: within 5 % of fp32's error).
+// The factor 2^14 keeps entries of all four matrices below 65504 (|X| <= 1.21, |A| <= 1.46, |P| <= 2.81) and lo above
+// the smallest fp16 number for entries down to 2^-13 of the largest.  a X stays outside the product, with X read back as
+// hi + lo: folding a into P's diagonal costs a factor of three in accuracy for nearly low-rank gradients.
+// For a bf16 result all steps but the last two take hi hi alone, a third of the work: the iteration contracts what
+// that costs (2^-12 per product), and 5 10^-5 to 8 10^-4 of |X| is left of it, under the 1.7 10^-3 of the result's own
+// rounding.  X itself keeps both parts in every step: with hi alone, gradients of low rank lose 4 10^-2.
 //
-// Layout: a matrix is rows of 128-byte groups, 32 columns each: 32 hi, then 32 lo.  A stage of the product (32 of k) is then
-// one 128-byte line per row, and the tile in LDS is the fp32 kernel's [row][32 words] with its swizzle (cn_gemm.hip).  All
-// sizes are padded to whole tiles with zeros, so nothing in the product needs a bounds check.  X is kept in both
-// orientations (the Gram product sums over n, the update over m), P and A are symmetric.
+// Layout: a matrix is blocks of 256 rows, in them groups of 32 columns: a 128-byte line per row, 32 hi, then 32 lo.  A stage of
+// the product is then one line (or two) per row, all of them in a row in memory, and the tile in LDS is the fp32 kernel's
+// [row][32 words] with its swizzle (cn_gemm.hip).  All sizes are padded to whole tiles with zeros, so nothing in the
+// product needs a bounds check.  X is kept in both orientations (the Gram product sums over n, the update over m), P
+// and A are symmetric.
 //
-// Work split: the tiles' stages, laid end to end, are dealt to W workgroups in equal contiguous runs, so the 136 tiles above the
-// diagonal of a 4096 x 4096 result load all compute units evenly.  A run that begins or ends inside a tile leaves a part of
-// that tile's sum; a second kernel adds a tile's parts in order, applies the formula and writes the next operand (both
-// orientations), so the result does not depend on scheduling.
+// Work split: see `Group` for how tiles go to workgroups, cost_of for which cut of a product is taken.  A workgroup that
+// computes a whole tile applies the formula to its accumulators and writes the next operand in both orientations; parts of a
+// tile go to memory and a second kernel adds them in order.  Either way the result does not depend on scheduling.
+//
+// Measured (one MI355X): X^T P of 4096 x 16384 in 1.34 ms, 1.23 PFLOP/s of fp16 products with the write-out of X and X^T in it
+// (0.8 GB, of which little overlaps); the library's own 8192^3 fp16 product reaches 1.31 on the same card.  The chip runs
+// at its power limit (1.75 GHz on random numbers, 2.1 on zeros), so what would be won by fewer stalls is lost in clock.
 #include "cn_dtypes.h"
 
 namespace cn {
@@ -47,9 +53,10 @@ constexpr int kStage = 32;                          // of k
 int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
 
 // ---- split numbers -----------------------------------------------------------------------------------------------------
-// Element (row, col) of a split matrix of `cols` columns: hi at row * 2 cols + (col / 32) * 64 + col % 32, lo 32 further.
+// Element (row, col) of a split matrix of `cols` columns: blocks of 256 rows, in them groups of 32 columns, in them the rows,
+// 64 numbers each: 32 hi, then 32 lo.  Returns the place of hi, lo is 32 further.
 __device__ __forceinline__ size_t split_at(int64_t row, int64_t col, int64_t cols) {
-    return (size_t)row * 2 * cols + (size_t)(col >> 5) * 64 + (col & 31);
+    return ((size_t)(row >> 8) * (size_t)(cols >> 5) + (size_t)(col >> 5)) * (256 * 64) + (size_t)(row & 255) * 64 + (col & 31);
 }
 // Four consecutive columns (col a multiple of 4), in stored units.
 __device__ __forceinline__ void split_store(f16_t *m, size_t at, const float (&v)[4]) {
@@ -164,28 +171,63 @@ __global__ __launch_bounds__(256) void split_kernel(Source s, const double *part
 }
 
 // ---- products ------------------------------------------------------------------------------------------------------------
-// D[i][j] = sum over k of U[i][k] V[j][k], both operands split.  `parts` receives TILE x TILE fp32 numbers per (tile, workgroup)
-// pair, at slot tile + workgroup: along a run either the tile or the workgroup moves on, so every part has a slot of its own.
+// D[i][j] = sum over k of U[i][k] V[j][k], both operands split, and what becomes of it.
+enum Finish {
+    GRAM = 0,  // A, symmetric
+    POLY = 1,  // P = b A + c A A, symmetric; D = A A
+    STEP = 2,  // X <- a X + P X, both orientations; D = X^T P, n x m
+    LAST = 3   // the same, into the result
+};
+//
+// Units of work: a group of `count` consecutive tiles, each cut along k into `parts`; workgroup w of a group takes part
+// w / count of tile first + (w % count) * rounds, and the rounds - 1 tiles behind it.  So the workgroups of an XCD, which take
+// neighbouring w, stream the same k of neighbouring tiles at the same time and share it in their L2.
+struct Group {
+    int first, count, parts, rounds, slot;  // slot: where its parts begin
+};
+constexpr int kMaxGroups = 4;
 struct Product {
     const f16_t *u, *v;
     int64_t u_cols, v_cols;  // columns of the split matrices (padded)
     int tiles_j;             // tiles along j
-    int tiles;               // all tiles; symmetric: those with j >= i
-    int symmetric;
     int stages;              // of k
-    float *parts;
+    int triangle;            // the result is symmetric: only tiles with j >= i
+    Group group[kMaxGroups];  // unused ones: all 0
+    float *parts;            // TILE x TILE numbers per unit of a group with more than one part per tile
+    const f16_t *old;        // POLY: A;  STEP, LAST: X
+    f16_t *to;               // GRAM, POLY: A, P;  STEP: X (its own elements only, so in place)
+    f16_t *to_t;             // STEP: X^T of the next step (this one's is an operand)
+    int64_t to_cols, to_t_cols;
+    void *out;               // LAST: the result, as the caller has it, or the weights
+    int out_dtype;
+    int64_t ldo, m, n;
+    int flip;                // the caller's matrix is n x m
+    int wide;                // its rows allow accesses of four numbers
+    int update;              // out = keep * out - rate * X
+    float keep, rate;
 };
 
+// TILE x TILE results of a workgroup: KS x WM x WN wavefronts of FM x FN blocks of 32 x 32, KS of them on the same blocks, each
+// with its share of a stage's k.  A stage is LINES 128-byte lines of every row (one where the products are of one part), DEPTH of
+// them are in LDS: 128 KiB in all, one workgroup per compute unit, so that what is in flight covers the way from the L2 even
+// where a stage has little to compute.  (64 x 64 with one line a stage: 0.31 us each, mostly the barrier's round trip.)
 template <int TILE> struct Shape;
-template <> struct Shape<256> { static constexpr int WM = 2, WN = 4, FM = 4, FN = 2; };  // wavefronts, 32 x 32 blocks of each
-template <> struct Shape<128> { static constexpr int WM = 2, WN = 2, FM = 2, FN = 2; };
-template <int TILE> constexpr int threads_of() { return Shape<TILE>::WM * Shape<TILE>::WN * 64; }
+template <> struct Shape<256> { static constexpr int KS = 1, WM = 2, WN = 4, FM = 4, FN = 2, LINES = 1, DEPTH = 2; };
+template <> struct Shape<128> { static constexpr int KS = 2, WM = 2, WN = 2, FM = 2, FN = 2, LINES = 2, DEPTH = 2; };
+template <> struct Shape<64> { static constexpr int KS = 2, WM = 2, WN = 2, FM = 1, FN = 1, LINES = 2, DEPTH = 4; };
+template <int TILE> constexpr int threads_of() { return Shape<TILE>::KS * Shape<TILE>::WM * Shape<TILE>::WN * 64; }
+template <int TILE> constexpr int lds_of() { return Shape<TILE>::DEPTH * Shape<TILE>::LINES * 2 * TILE * 128 + threads_of<TILE>() * 64; }
+constexpr int lines_of(int tile, int terms) {
+    return terms == 1 ? 1 : tile == 256 ? Shape<256>::LINES : tile == 128 ? Shape<128>::LINES : Shape<64>::LINES;
+}
+// k of a stage.
+constexpr int depth_of(int tile, int terms) { return lines_of(tile, terms) * (terms == 3 ? 32 : 64); }
 
 __device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ ((row >> 3) & 3); }
 
 // Tile number to its row and column of tiles; symmetric: row by row, each from the diagonal on.
-__device__ __forceinline__ void tile_place(int tile, int tiles_j, int symmetric, int &ti, int &tj) {
-    if (!symmetric) {
+__device__ __forceinline__ void tile_place(int tile, int tiles_j, bool triangle, int &ti, int &tj) {
+    if (!triangle) {
         ti = tile / tiles_j;
         tj = tile - ti * tiles_j;
         return;
@@ -199,247 +241,553 @@ __device__ __forceinline__ void tile_place(int tile, int tiles_j, int symmetric,
     tj = ti + left;
 }
 
-template <int TILE>
-__global__ __launch_bounds__(threads_of<TILE>(), 2) void product_kernel(Product g) {
+// The units of this workgroup, one per group: lane g of every wavefront finds and keeps that of group g.
+struct Units {
+    int tile;    // ti * 65536 + tj
+    int stages;  // begin * 65536 + end
+    int slot;    // < 0: whole tiles
+    int rounds;  // 0: the group has no unit for this workgroup
+    __device__ __forceinline__ Units(const Product &g, int w) {
+        tile = stages = slot = rounds = 0;
+        const int lane = threadIdx.x & 63;
+        if (lane < kMaxGroups) {
+            const Group a = g.group[lane];
+            if (w < a.count * a.parts) {
+                const int part = w / a.count, place = w - part * a.count;
+                int ti, tj;
+                tile_place(a.first + place * a.rounds, g.tiles_j, g.triangle, ti, tj);
+                tile = ti << 16 | tj;
+                stages = g.stages * part / a.parts << 16 | g.stages * (part + 1) / a.parts;
+                slot = a.parts > 1 ? a.slot + w : -1;
+                rounds = a.rounds;
+            }
+        }
+    }
+};
+// What a workgroup is at: a stage of a unit.  All of it the same for every lane.
+struct Cursor {
+    int group = -1, ti = 0, tj = 0, stage = 0, end = 0, slot = 0, rounds = 0;
+    __device__ __forceinline__ bool next_unit(const Product &g, const Units &u) {
+        if (rounds > 1) {  // the next tile, all of it
+            --rounds;
+            stage = 0;
+            if (++tj == g.tiles_j) {
+                ++ti;
+                tj = g.triangle ? ti : 0;
+            }
+            return true;
+        }
+#pragma unroll 1
+        while (++group < kMaxGroups) {
+            rounds = __builtin_amdgcn_readlane(u.rounds, group);
+            if (rounds == 0) continue;
+            const int tile = __builtin_amdgcn_readlane(u.tile, group), stages = __builtin_amdgcn_readlane(u.stages, group);
+            ti = tile >> 16;
+            tj = tile & 0xffff;
+            stage = stages >> 16;
+            end = stages & 0xffff;
+            slot = __builtin_amdgcn_readlane(u.slot, group);
+            return true;
+        }
+        return false;
+    }
+};
+
+// What a lane needs of the old X or A for a 32 x 32 block: rows j, along i.
+struct Old {
+    f16x4 hi[4], lo[4];
+};
+template <int FINISH>
+__device__ __forceinline__ void load_old(const Product &g, int64_t i0, int64_t j0, Old &o) {
+    if (FINISH == GRAM) return;
+    const int sub = (threadIdx.x & 63) >> 3, quad = threadIdx.x & 7;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const f16_t *at = g.old + split_at(j0 + 8 * p + sub, i0 + 4 * quad, g.to_cols);
+        o.hi[p] = *reinterpret_cast<const f16x4 *>(at);
+        o.lo[p] = *reinterpret_cast<const f16x4 *>(at + 32);
+    }
+}
+
+// Four numbers of the result, along a row of the caller's matrix.
+__device__ __forceinline__ void write_result(const Product &g, int64_t row, int64_t col, const float (&x)[4]) {
+    const int64_t rows = g.flip ? g.n : g.m, cols = g.flip ? g.m : g.n, at = row * g.ldo + col;
+    if (row >= rows) return;
+    if (g.wide && col + 4 <= cols) {
+        float w[4] = {x[0], x[1], x[2], x[3]};
+        if (g.out_dtype == CN_F32) {
+            float *out = (float *)g.out + at;
+            if (g.update) {
+                float old[4];
+                load_f32<4>(out, old);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = g.keep * old[e] - g.rate * w[e];
+            }
+            store_f32<4>(out, w);
+        } else if (g.out_dtype == CN_F16) {
+            store_f32<4>((f16_t *)g.out + at, w);
+        } else {
+            store_f32<4>((bf16_t *)g.out + at, w);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (col + e >= cols) break;
+        if (g.out_dtype == CN_F32) {
+            float *out = (float *)g.out + at + e;
+            *out = g.update ? g.keep * *out - g.rate * x[e] : x[e];
+        } else if (g.out_dtype == CN_F16) {
+            ((f16_t *)g.out)[at + e] = (f16_t)x[e];
+        } else {
+            ((bf16_t *)g.out)[at + e] = (bf16_t)x[e];
+        }
+    }
+}
+
+// One 32 x 32 block of D, corner (i0, j0), from a wavefront's sums as the matrix instructions leave them: number r of lane
+// (half, l) is row 8 (r / 4) + 4 half + r % 4, column l.  X, A and P are read and written as rows j, along i (A, A A and P are
+// symmetric, D = X^T P belongs to row j of X), then, with `mirror`, as rows i, along j.  `stage`: 4 KiB of LDS of the
+// wavefront's own, [j][i] in 16-byte columns xor-swizzled by j / 2, so that eight lanes write 64 bytes of a row at a time.
+template <int FINISH>
+__device__ __forceinline__ void finish_block(const Product &g, const f32x16 &sum, const Old &old, int64_t i0, int64_t j0, bool mirror,
+                                             float *stage) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4 *>(stage + l32 * 32 + (((2 * q + half) ^ (l32 >> 1)) & 7) * 4) =
+            f32x4{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]};
+    __builtin_amdgcn_wave_barrier();
+    const int sub = lane >> 3, quad = lane & 7;
+    constexpr bool last = FINISH == LAST;
+    const float x = FINISH == POLY ? kB : kA, y = (FINISH == POLY ? kC : 1.0f) * (kProduct * kUnit);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const int j = 8 * p + sub;
+        f32x4 *at = reinterpret_cast<f32x4 *>(stage + j * 32 + ((quad ^ (j >> 1)) & 7) * 4);
+        f32x4 v = *at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] *= y;
+            if (FINISH != GRAM) v[e] = x * ((float)old.hi[p][e] + (float)old.lo[p][e]) + v[e];
+        }
+        const float w[4] = {v[0], v[1], v[2], v[3]};
+        if (!last) {
+            split_store(g.to, split_at(j0 + j, i0 + 4 * quad, g.to_cols), w);
+        } else if (!g.flip) {
+            const float r[4] = {w[0] * (1.0f / kUnit), w[1] * (1.0f / kUnit), w[2] * (1.0f / kUnit), w[3] * (1.0f / kUnit)};
+            write_result(g, j0 + j, i0 + 4 * quad, r);
+        }
+        *at = v;
+    }
+    if (last ? !g.flip : !mirror) return;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const int i = 8 * p + sub;
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int j = 4 * quad + e;
+            w[e] = stage[j * 32 + (((i >> 2) ^ (j >> 1)) & 7) * 4 + (i & 3)];
+            if (last) w[e] *= 1.0f / kUnit;
+        }
+        if (last) write_result(g, i0 + i, j0 + 4 * quad, w);
+        else split_store(FINISH == STEP ? g.to_t : g.to, split_at(i0 + i, j0 + 4 * quad, g.to_t_cols), w);
+    }
+}
+
+template <int N> struct Constant { static constexpr int value = N; };
+// f(Constant<0>) ... f(Constant<N - 1>): registers can only be named by constants.
+template <int N, typename F>
+__device__ __forceinline__ void for_each(F &&f) {
+    if constexpr (N > 0) {
+        for_each<N - 1>(f);
+        f(Constant<N - 1>{});
+    }
+}
+
+template <int COUNT>
+__device__ __forceinline__ void wait_for_all_but() {  // vmcnt(COUNT)
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (COUNT & 15) | ((COUNT >> 4) << 14));
+}
+
+// TERMS = 3: hi hi + hi lo + lo hi, a stage is 32 of k.  TERMS = 1: hi hi alone, a stage is 64 of k, the hi halves of two
+// groups, in the same place in LDS.
+template <int TILE, int TERMS, int FINISH>
+__global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product g) {
     using S = Shape<TILE>;
-    constexpr int kWaves = S::WM * S::WN, kLoads = TILE / 8 / kWaves;  // 1 KiB loads per operand, stage and wavefront
-    extern __shared__ __attribute__((aligned(16))) char smem[];         // [2 stages][U, V][TILE rows][128 bytes]
-    constexpr int kOperand = TILE * 128;
+    constexpr int kWaves = S::KS * S::WM * S::WN, kLines = lines_of(TILE, TERMS);
+    constexpr int kLoads = kLines * TILE / 8 / kWaves;  // 1 KiB loads per operand, stage and wavefront
+    extern __shared__ __attribute__((aligned(16))) char smem[];         // [DEPTH][U, V][line][TILE rows][128 bytes], then 4 KiB per wavefront
+    constexpr int kOperand = S::LINES * TILE * 128, kMask = S::DEPTH - 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int half = lane >> 5, l32 = lane & 31;
-    const int wave_i = wave / S::WN, wave_j = wave % S::WN;
+    const int share = wave / (S::WM * S::WN), wave_i = wave % (S::WM * S::WN) / S::WN, wave_j = wave % S::WN;
 
     // Workgroups of one XCD (ids congruent mod 8) take neighbouring runs and share operands in its L2.
     const unsigned W = gridDim.x, xcd = blockIdx.x % 8u, idx = blockIdx.x / 8u, per = W / 8u, rem = W % 8u;
     const int w = (int)(xcd * per + (xcd < rem ? xcd : rem) + idx);
-    const int64_t total = (int64_t)g.tiles * g.stages;
-    const int64_t u0 = total * w / (int)W, u1 = total * (w + 1) / (int)W;
-    if (u0 >= u1) return;
-    int tile = __builtin_amdgcn_readfirstlane((int)(u0 / g.stages));
-    int stage = __builtin_amdgcn_readfirstlane((int)(u0 % g.stages));
-    int left = __builtin_amdgcn_readfirstlane((int)(u1 - u0));
-    int ti, tj;
-    tile_place(tile, g.tiles_j, g.symmetric, ti, tj);
+    const Units units(g, w);
+    Cursor at, ahead;  // the stage that is computed, the one that is requested next
+    bool more = ahead.next_unit(g, units);  // something is left to request
+    int requested = 0;                      // stages requested and not yet computed
 
-    uint32_t off_u[kLoads], off_v[kLoads];  // this lane's 16 bytes of each 1 KiB (8 rows), from the tile's corner
+    uint32_t off[kLoads];  // this lane's 16 bytes of each 1 KiB (8 rows), from the corner of the tile's stage
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-        const int row = (j * kWaves + wave) * 8 + (lane >> 3);
-        const uint32_t quad = (uint32_t)(((lane & 7) ^ swizzle(row)) * 16);
-        off_u[j] = (uint32_t)row * (uint32_t)(g.u_cols * 4) + quad;
-        off_v[j] = (uint32_t)row * (uint32_t)(g.v_cols * 4) + quad;
+        const int at = (j * kWaves + wave) * 8 + (lane >> 3), row = at % TILE;
+        const uint32_t column = (uint32_t)((lane & 7) ^ swizzle(row));
+        off[j] = (uint32_t)(at / TILE) * (256 * 128) + (uint32_t)row * 128 + (TERMS == 3 ? column * 16 : (column >> 2) * (256 * 128) + (column & 3) * 16);
     }
     // Inline assembly because the compiler would make every later LDS read wait for a load it knows to write LDS; the wait
-    // is at the end of each stage.  No output registers.
-    auto issue_one = [&](const f16_t *corner, const uint32_t (&off)[kLoads], int lds) {
-        const uint64_t addr = reinterpret_cast<uint64_t>(corner);
+    // is at the head of each stage.  No output registers.
+    constexpr uint32_t kStep = depth_of(TILE, TERMS) / 32 * 256 * 128;  // bytes from a stage's corner to the next one's
+    const uint32_t lds_first = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)smem) + (uint32_t)(wave * 1024);
+    uint64_t next_u = 0, next_v = 0;  // corners of the stage that is requested next
+    auto aim = [&]() {
+        const int64_t column = (int64_t)ahead.stage * depth_of(TILE, TERMS);
+        next_u = reinterpret_cast<uint64_t>(g.u + split_at((int64_t)ahead.ti * TILE, column, g.u_cols));
+        next_v = reinterpret_cast<uint64_t>(g.v + split_at((int64_t)ahead.tj * TILE, column, g.v_cols));
+    };
+    auto issue_one = [&](uint64_t addr, uint32_t lds) {
         const u32x4 rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)addr),
                             (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(addr >> 32)) & 0xffffu, 0xffffffffu, 0x00020000u};
-        const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)smem) +
-                              (uint32_t)(lds + wave * 1024);
 #pragma unroll
         for (int j = 0; j < kLoads; ++j)
             asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
-                         : "s"(lds0 + (uint32_t)(j * kWaves) * 1024u), "v"(off[j]), "s"(rsrc)
+                         : "s"(lds + (uint32_t)(j * kWaves) * 1024u), "v"(off[j]), "s"(rsrc)
                          : "memory", "m0");
     };
-    auto issue = [&](int ti_, int tj_, int stage_, int slot) {
-        issue_one(g.u + (int64_t)ti_ * TILE * 2 * g.u_cols + (int64_t)stage_ * 64, off_u, slot * 2 * kOperand);
-        issue_one(g.v + (int64_t)tj_ * TILE * 2 * g.v_cols + (int64_t)stage_ * 64, off_v, slot * 2 * kOperand + kOperand);
+    int ahead_slot = 0;
+    auto issue = [&]() {
+        const uint32_t lds = lds_first + (uint32_t)ahead_slot * (2 * kOperand);
+        issue_one(next_u, lds);
+        issue_one(next_v, lds + kOperand);
+        ahead_slot = (ahead_slot + 1) & kMask;
+        ++requested;
+        next_u += kStep;
+        next_v += kStep;
+        if (++ahead.stage == ahead.end) {
+            more = ahead.next_unit(g, units);
+            if (more) aim();
+        }
     };
+    aim();
 
     f32x16 acc[S::FM][S::FN];
 
     // Lane (half, i) reads k = 16 s + 8 half .. + 7 of row i: 16-byte column 2 s + half of its row, lo four columns further.
+    constexpr int kSteps = TERMS == 3 ? 2 : 4;
     auto frag = [&](int base, int row, int quad) {
         return *reinterpret_cast<const f16x8 *>(smem + base + row * 128 + ((quad ^ swizzle(row)) << 4));
     };
-    auto compute = [&](int slot) {
-        const int bu = slot * 2 * kOperand, bv = bu + kOperand;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            f16x8 uh[S::FM], ul[S::FM], vh[S::FN], vl[S::FN];
+    // KS == 1: a stage is kSteps x FM groups of matrix instructions, one block row of the wavefront at one s each; a group's
+    // operands are read from LDS while the group before it computes, the first group's of a stage behind the barrier that
+    // publishes it, which sits before the last group of the stage before.  (With all of a step's reads in front of its
+    // instructions the wavefronts, in step after the barrier, took turns between LDS and matrix cores: 4400 cycles a stage
+    // of 256 x 256 x 32 instead of 3072.)
+    constexpr int kGroups = kSteps * S::FM;
+    static_assert(S::KS > 1 || kGroups % 2 == 0, "the buffers alternate across stages");
+    f16x8 uh[2], ul[2], vh[2][S::FN], vl[2][S::FN];
+    auto read_group = [&](int slot, int group) {  // into buffer group % 2 (U) and s % 2 (V)
+        const int bu = slot * 2 * kOperand, bv = bu + kOperand, s = group / S::FM, mi = group % S::FM;
+        if (mi == 0) {
 #pragma unroll
             for (int ni = 0; ni < S::FN; ++ni) {
                 const int row = (wave_j * S::FN + ni) * 32 + l32;
-                vh[ni] = frag(bv, row, 2 * s + half);
-                vl[ni] = frag(bv, row, 4 + 2 * s + half);
+                vh[s & 1][ni] = frag(bv, row, 2 * s + half);
+                if (TERMS == 3) vl[s & 1][ni] = frag(bv, row, 4 + 2 * s + half);
+            }
+        }
+        const int row = (wave_i * S::FM + mi) * 32 + l32;
+        uh[group & 1] = frag(bu, row, 2 * s + half);
+        if (TERMS == 3) ul[group & 1] = frag(bu, row, 4 + 2 * s + half);
+    };
+    auto multiply_group = [&](int group) {
+        const int s = group / S::FM, mi = group % S::FM;
+#pragma unroll
+        for (int term = 3 - TERMS; term < 3; ++term)
+#pragma unroll
+            for (int ni = 0; ni < S::FN; ++ni)
+                acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_f16(term == 0 ? ul[group & 1] : uh[group & 1],
+                                                                     term == 1 ? vl[s & 1][ni] : vh[s & 1][ni], acc[mi][ni], 0, 0, 0);
+    };
+    // KS == 2: a wavefront's half of the stage's steps at once; the other wavefronts of its SIMD cover the reads.
+    auto compute = [&](int slot, auto request) {
+        // two lines: one for each half of the wavefronts; one line: half of its steps
+        constexpr int kMySteps = kSteps * kLines / S::KS;
+        const int bu = slot * 2 * kOperand + (kLines == 2 ? share * TILE * 128 : 0), bv = bu + kOperand;
+#pragma unroll
+        for (int q = 0; q < kMySteps; ++q) {
+            const int column = 2 * ((kLines == 2 ? 0 : share * kMySteps) + q) + half;
+            f16x8 ah[S::FM], al[S::FM], bh[S::FN], bl[S::FN];
+#pragma unroll
+            for (int ni = 0; ni < S::FN; ++ni) {
+                const int row = (wave_j * S::FN + ni) * 32 + l32;
+                bh[ni] = frag(bv, row, column);
+                if (TERMS == 3) bl[ni] = frag(bv, row, 4 + column);
             }
 #pragma unroll
             for (int mi = 0; mi < S::FM; ++mi) {
                 const int row = (wave_i * S::FM + mi) * 32 + l32;
-                uh[mi] = frag(bu, row, 2 * s + half);
-                ul[mi] = frag(bu, row, 4 + 2 * s + half);
+                ah[mi] = frag(bu, row, column);
+                if (TERMS == 3) al[mi] = frag(bu, row, 4 + column);
             }
+            if (q == 0) request();  // its address arithmetic runs while the operands are on their way
 #pragma unroll
-            for (int term = 0; term < 3; ++term)
+            for (int term = 3 - TERMS; term < 3; ++term)
 #pragma unroll
                 for (int mi = 0; mi < S::FM; ++mi)
 #pragma unroll
                     for (int ni = 0; ni < S::FN; ++ni)
-                        acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_f16(term == 0 ? ul[mi] : uh[mi], term == 1 ? vl[ni] : vh[ni],
+                        acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_f16(term == 0 ? al[mi] : ah[mi], term == 1 ? bl[ni] : bh[ni],
                                                                              acc[mi][ni], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    issue(ti, tj, stage, 0);
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the stage is in LDS
-    __syncthreads();
+    // Stages are requested into every slot up front and then, stage by stage, into the slot that was read last.
+#pragma unroll 1
+    for (int d = 0; d < S::DEPTH - (S::KS > 1 ? 1 : 0) && more; ++d) issue();
     int slot = 0;
-    while (left > 0) {  // a tile, or as much of it as the run holds
-        const int here = left < g.stages - stage ? left : g.stages - stage;
-        left -= here;
-        int ni = ti, nj = tj + 1;
-        if (nj == g.tiles_j) {
-            ++ni;
-            nj = g.symmetric ? ni : 0;
-        }
+    bool counted = true;  // only stage loads are outstanding
+    if (S::KS == 1) {
+        if (requested == S::DEPTH) wait_for_all_but<(S::DEPTH - 1) * 2 * kLoads>();
+        else wait_for_all_but<0>();
+        __syncthreads();
+        read_group(0, 0);
+    }
+    while (at.next_unit(g, units)) {
 #pragma unroll
         for (int mi = 0; mi < S::FM; ++mi)
 #pragma unroll
             for (int n = 0; n < S::FN; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[mi][n][r] = 0.0f;
-        for (int i = 1; i <= here; ++i) {  // the loads of the next stage, of this tile or the next, run under this one's products
-            if (i < here) issue(ti, tj, stage + i, slot ^ 1);
-            else if (left > 0) issue(ni, nj, 0, slot ^ 1);
-            compute(slot);
-            __builtin_amdgcn_s_waitcnt(0x0f70);
-            __syncthreads();
-            slot ^= 1;
+        for (; at.stage < at.end; ++at.stage) {
+            if constexpr (S::KS == 1) {
+#pragma unroll
+                for (int group = 0; group + 1 < kGroups; ++group) {
+                    read_group(slot, group + 1);
+                    multiply_group(group);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (requested > 1) {
+                    wait_for_all_but<0>();  // the next stage has landed
+                    __syncthreads();        // for every wavefront's loads; and everyone has read the last of this stage
+                    slot = (slot + 1) & kMask;
+                    read_group(slot, 0);
+                    if (more) issue();  // into the slot of the stage before
+                }
+                --requested;
+                multiply_group(kGroups - 1);
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                // this stage has landed when at most the DEPTH - 2 younger ones are outstanding
+                if (S::DEPTH > 2 && counted && requested == S::DEPTH - 1) wait_for_all_but<(S::DEPTH - 2) * 2 * kLoads>();
+                else wait_for_all_but<0>();
+                counted = true;
+                __syncthreads();  // for every wavefront's loads, and everyone is done with the slot that is filled next
+                compute(slot, [&]() {
+                    if (more) issue();
+                });
+                slot = (slot + 1) & kMask;
+                --requested;
+            }
         }
-        float *out = g.parts + (size_t)(tile + w) * TILE * TILE + (wave_i * S::FM * 32 + 4 * half) * TILE + wave_j * S::FN * 32 + l32;
+        counted = false;
+        float *own = reinterpret_cast<float *>(smem + S::DEPTH * 2 * kOperand) + wave * 1024;
+        constexpr int kBlocks = S::FM * S::FN, kMine = (kBlocks + S::KS - 1) / S::KS;
+        if constexpr (S::KS == 2) {
+            // the two halves meet: each wavefront of a pair takes half of their blocks (the first one a single block)
+            const float *theirs = own + (share ? -1 : 1) * (S::WM * S::WN * 1024);
+            auto exchange = [&](auto first, auto second) {  // block this wavefront gives, block it takes
+                constexpr int give = decltype(first)::value, take = decltype(second)::value;
+                if constexpr (give < kBlocks) {
 #pragma unroll
-        for (int mi = 0; mi < S::FM; ++mi)
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x16 &a = acc[give / S::FN][give % S::FN];
+                        *reinterpret_cast<f32x4 *>(own + q * 256 + lane * 4) = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+                    }
+                }
+                __syncthreads();
+                if constexpr (take < kBlocks) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x4 x = *reinterpret_cast<const f32x4 *>(theirs + q * 256 + lane * 4);
 #pragma unroll
-                for (int n = 0; n < S::FN; ++n) out[(mi * 32 + 8 * (r >> 2) + (r & 3)) * TILE + n * 32] = acc[mi][n][r];
-        stage = 0;
-        ++tile;
-        ti = ni;
-        tj = nj;
+                        for (int e = 0; e < 4; ++e) acc[take / S::FN][take % S::FN][4 * q + e] += x[e];
+                    }
+                }
+                __syncthreads();
+            };
+            if (share == 0) {
+                exchange(Constant<kMine>{}, Constant<0>{});
+                if constexpr (kMine > 1) exchange(Constant<kMine + 1>{}, Constant<1>{});
+            } else {
+                exchange(Constant<0>{}, Constant<kMine>{});
+                if constexpr (kMine > 1) exchange(Constant<1>{}, Constant<kMine + 1>{});
+            }
+        }
+        // a finished block, or its part of the sum as the registers lie: [32 x 32 block][number / 4][lane][4]
+        const bool mirror = !(g.triangle && at.ti == at.tj);
+        auto place_i = [&](int b) { return (int64_t)at.ti * TILE + (wave_i * S::FM + b / S::FN) * 32; };
+        auto place_j = [&](int b) { return (int64_t)at.tj * TILE + (wave_j * S::FN + b % S::FN) * 32; };
+        const int from = share * kMine, until = from + kMine < kBlocks ? from + kMine : kBlocks;
+        // One copy of the code for all blocks (unrolled it would be most of the kernel, fetched anew by every launch): the block's
+        // registers are picked by a branch.  Old values are requested a block ahead, in front of the stores of the block before:
+        // the counter that a load is waited for with would otherwise drain them first.
+        Old old, next;
+        if (at.slot < 0 && from < until) load_old<FINISH>(g, place_i(from), place_j(from), old);
+#pragma unroll 1
+        for (int b = from; b < until; ++b) {
+            f32x16 sum;
+            for_each<kBlocks>([&](auto step) {
+                constexpr int k = decltype(step)::value;
+                if (b == k) {
+                    sum = acc[k / S::FN][k % S::FN];
+                    asm volatile("" : "+v"(sum));  // a branch, not sixteen selects for every block
+                }
+            });
+            if (at.slot < 0) {
+                if (b + 1 < until) load_old<FINISH>(g, place_i(b + 1), place_j(b + 1), next);
+                finish_block<FINISH>(g, sum, old, place_i(b), place_j(b), mirror, own);
+                old = next;
+            } else {
+                float *out = g.parts + (size_t)at.slot * TILE * TILE;
+                const int block = (wave_i * S::FM + b / S::FN) * (TILE / 32) + wave_j * S::FN + b % S::FN;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4 *>(out + block * 1024 + q * 256 + lane * 4) =
+                        f32x4{sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]};
+            }
+        }
     }
 }
 
-// ---- what becomes of a product --------------------------------------------------------------------------------------------
-enum Finish {
-    GRAM = 0,  // A
-    POLY = 1,  // P = b A + c A A
-    STEP = 2,  // X <- a X + P X, both orientations
-    LAST = 3   // the same, into the result
-};
-struct FinishArgs {
-    const float *parts;
-    int tile, tiles_j, symmetric, stages, workgroups;
-    int64_t total;           // tiles * stages
-    const f16_t *old;        // POLY: A;  STEP, LAST: X^T
-    int64_t cols;            // columns of D's split form: mp
-    f16_t *to, *to_t;        // D's split form and its transpose's (GRAM, POLY: the same matrix, mirrored)
-    int64_t cols_t;
-    // LAST
-    void *out;               // the result, rows x cols as the caller has it (fp32 or 16 bits), or the weights (fp32)
-    int64_t ldo, m, n;       // D is n x m
-    int flip;                // the caller's matrix is n x m
-    int update;              // out = keep * out - rate * X
-    float keep, rate;
-};
-
-template <int MODE, typename E>
-__global__ __launch_bounds__(256) void finish_kernel(FinishArgs g) {
-    __shared__ float mirror[64][65];
-    const int per_side = g.tile / 64;
-    const int tile = blockIdx.x / (per_side * per_side), block = blockIdx.x % (per_side * per_side);
+// The tiles of groups with several parts: the parts are added in order.  A wavefront takes a 32 x 32 block.
+template <int TILE, int FINISH>
+__global__ __launch_bounds__(256) void join_kernel(Product g, int from) {
+    __shared__ __attribute__((aligned(16))) float stage[4][1024];
+    constexpr int kSide = TILE / 32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int tile = from + blockIdx.x / (kSide * kSide / 4), block = blockIdx.x % (kSide * kSide / 4) * 4 + wave;
+    Group a = g.group[0];
+#pragma unroll
+    for (int i = 1; i < kMaxGroups; ++i)
+        if (g.group[i].count > 0 && tile >= g.group[i].first) a = g.group[i];
+    if (a.parts < 2) return;
     int ti, tj;
-    tile_place(tile, g.tiles_j, g.symmetric, ti, tj);
-    const int bi = block / per_side * 64, bj = block % per_side * 64;
-    const int64_t i0 = (int64_t)ti * g.tile + bi, j0 = (int64_t)tj * g.tile + bj;
-    // the workgroups whose runs touch this tile: w holds units total * w / W .. total * (w + 1) / W - 1
-    const int64_t first = (int64_t)tile * g.stages, last = first + g.stages - 1;
-    const int w0 = (int)(((first + 1) * g.workgroups - 1) / g.total), w1 = (int)(((last + 1) * g.workgroups - 1) / g.total);
-    const int row = threadIdx.x >> 4, col = (threadIdx.x & 15) * 4;
-    float v[4][4];
+    tile_place(tile, g.tiles_j, g.triangle, ti, tj);
+    const int64_t i0 = (int64_t)ti * TILE + block / kSide * 32, j0 = (int64_t)tj * TILE + block % kSide * 32;
+    Old old;
+    load_old<FINISH>(g, i0, j0, old);
+    f32x16 sum;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[q][e] = 0.0f;
-    for (int w = w0; w <= w1; ++w) {
-        const float *p = g.parts + (size_t)(tile + w) * g.tile * g.tile + (size_t)(bi + row) * g.tile + bj + col;
+    for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
+    for (int part = 0; part < a.parts; ++part) {
+        const float *p = g.parts + (size_t)(a.slot + part * a.count + tile - a.first) * TILE * TILE + block * 1024 + lane * 4;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(p + (size_t)(16 * q) * g.tile);
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(p + q * 256);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[q][e] += x[e];
+            for (int e = 0; e < 4; ++e) sum[4 * q + e] += x[e];
         }
     }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int i = row + 16 * q;
-        const size_t at = split_at(i0 + i, j0 + col, g.cols);
-        if (MODE == GRAM) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[q][e] *= kProduct * kUnit;
-        } else {
-            float old[4];
-            split_load(g.old, at, old);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (MODE == POLY) v[q][e] = kB * old[e] + (kC * kProduct * kUnit) * v[q][e];
-                else v[q][e] = kA * old[e] + (kProduct * kUnit) * v[q][e];
-            }
-        }
-        if (MODE != LAST) split_store(g.to, at, v[q]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mirror[i][col + e] = v[q][e];
-    }
-    if (MODE == LAST) {
-        __syncthreads();
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 4
-        for (int q = 0; q < 16; ++q) {
-            const int a = wave + 4 * q;
-            // D[i][j] = X[j][i]; written along the rows of the caller's matrix
-            const int64_t r = (g.flip ? i0 : j0) + a, c = (g.flip ? j0 : i0) + lane;
-            if (r >= (g.flip ? g.n : g.m) || c >= (g.flip ? g.m : g.n)) continue;
-            const float x = (g.flip ? mirror[a][lane] : mirror[lane][a]) * (1.0f / kUnit);
-            E *out = (E *)g.out + r * g.ldo + c;
-            *out = (E)(g.update ? g.keep * (float)*out - g.rate * x : x);
-        }
-        return;
-    }
-    if (g.symmetric && ti == tj) return;  // a tile on the diagonal holds both halves
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int j = row + 16 * q;
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = mirror[col + e][j];
-        split_store(g.to_t, split_at(j0 + j, i0 + col, g.cols_t), x);
-    }
+    finish_block<FINISH>(g, sum, old, i0, j0, !(g.triangle && ti == tj), stage[wave]);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-// Tiles of 256 x 256 feed every matrix instruction from fewer LDS and L2 bytes; tiles of 128 x 128 spread small products
-// over more compute units.
-int tile_for(int64_t mp, int64_t np) { return mp * np >= (int64_t)2048 * 2048 ? 256 : 128; }
-int workgroups_for(int tile, int64_t total) {
-    const int most = tile == 256 ? 256 : 512;
-    const int64_t w = total / 4;  // at least four stages each
-    return (int)(w < 1 ? 1 : w > most ? most : w);
+// How a product is cut.
+struct Cut {
+    int tile, workgroups, tiles, tiles_j, stages;
+    int groups, slots;
+    Group group[kMaxGroups];
+    int whole;  // tiles before the first group with parts
+};
+constexpr int kSlots = 256;  // workgroups at a time, one per compute unit
+Cut cut_with(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, int terms, int tile, bool whole) {
+    Cut c{};
+    const int64_t ti = (rows_i + tile - 1) / tile, tj = (rows_j + tile - 1) / tile;
+    c.tile = tile;
+    c.tiles_j = (int)tj;
+    c.tiles = (int)(triangle ? tj * (tj + 1) / 2 : ti * tj);
+    c.stages = (int)((depth + depth_of(tile, terms) - 1) / depth_of(tile, terms));
+    auto add = [&](int count, int parts, int rounds) {
+        const int first = c.groups ? c.group[c.groups - 1].first + c.group[c.groups - 1].count * c.group[c.groups - 1].rounds : 0;
+        c.group[c.groups++] = Group{first, count, parts, rounds, c.slots};
+        if (parts > 1) c.slots += count * parts;
+        if (count * parts > c.workgroups) c.workgroups = count * parts;
+        if (c.slots == 0) c.whole += count * rounds;
+    };
+    int left = c.tiles;
+    if (left >= kSlots) {
+        add(kSlots, 1, left / kSlots);
+        left %= kSlots;
+    }
+    if (whole) {
+        if (left) add(left, 1, 1);
+        return c;
+    }
+    const int least = tile == 256 ? 8 : 4, most = c.stages / least < 1 ? 1 : c.stages / least;  // a part has `least` stages or more
+    while (left > 0) {
+        const bool final = c.groups + 1 == kMaxGroups;
+        int parts = final ? kSlots / left : (kSlots + left - 1) / left;
+        if (parts > most) parts = most;
+        if (parts < 1) parts = 1;
+        const int count = kSlots / parts < left ? kSlots / parts : left;
+        add(count, parts, 1);
+        left -= count;
+    }
+    return c;
+}
+// The time a cut is expected to take, in microseconds: what its workgroups do one after the other, and the join.  Measured on
+// 784 x 1024, 1000 x 4001, 4096 x 4096 and 4096 x 16384: a stage's time by tile size and parts per operand, a tile's
+// epilogue, storing a part; a launch takes 4 us more than what runs in it, the parts are written and read at about 8 TB/s together.
+double cost_of(const Cut &c, int terms) {
+    const int size = c.tile == 256 ? 0 : c.tile == 128 ? 1 : 2;
+    static const double stage[3][2] = {{2.1, 2.42}, {1.2, 1.55}, {0.55, 0.53}};  // [size][parts of the operands]
+    static const double finish[3] = {13.0, 3.0, 1.5}, store[3] = {3.0, 2.0, 1.0};
+    double t = 4.0;
+    int busy = 0;
+    for (const Group &g : c.group) {
+        if (g.count == 0) continue;
+        // a chip that is not full runs at a higher clock
+        const double one = stage[size][terms == 3] * (size < 2 && g.count * g.parts < 200 ? 0.72 : 1.0);
+        t += g.rounds * (c.stages / (double)g.parts * one + (g.parts > 1 ? store[size] : finish[size]));
+        busy += g.parts > 1 ? g.count * g.parts : 0;
+    }
+    if (busy) t += 4.5 + (double)busy * c.tile * c.tile * 8 / 8e6;
+    return t;
+}
+Cut cut_product(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, int terms) {
+    Cut best{};
+    double least = 0.0;
+    for (int tile : {256, 128, 64})
+        for (bool whole : {true, false}) {
+            const Cut c = cut_with(rows_i, rows_j, depth, triangle, terms, tile, whole);
+            const double t = cost_of(c, terms);
+            if (best.tile == 0 || t < least) {
+                best = c;
+                least = t;
+            }
+        }
+    return best;
 }
 
 struct Space {
-    f16_t *x, *xt, *a, *p;
+    f16_t *x, *xt[2], *a, *p;
     float *parts;
     double *norms;
     size_t bytes;
 };
+constexpr int kGram = 0, kSquare = 1, kApply = 2;  // the products of a step
 struct Sizes {
     int64_t m, n, mp, np;
-    int flip, tile;
+    int flip;
+    Cut cut[2][3];  // [products of one part, of three][product]
 };
 Sizes sizes_of(int64_t rows, int64_t cols) {
     Sizes z;
@@ -448,42 +796,56 @@ Sizes sizes_of(int64_t rows, int64_t cols) {
     z.n = z.flip ? rows : cols;
     z.mp = padded(z.m);
     z.np = padded(z.n);
-    z.tile = tile_for(z.mp, z.np);
+    for (int t = 0; t < 2; ++t) {
+        const int terms = t == 0 ? 1 : 3;
+        z.cut[t][kGram] = cut_product(z.m, z.m, z.n, true, terms);
+        z.cut[t][kSquare] = cut_product(z.m, z.m, z.m, true, terms);
+        z.cut[t][kApply] = cut_product(z.n, z.m, z.m, false, terms);
+    }
     return z;
 }
-int64_t tiles_along(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
 Space lay_out(void *workspace, const Sizes &z) {
     Carver c(workspace);
     Space s;
     s.x = c.take<f16_t>((size_t)z.mp * z.np * 2);
-    s.xt = c.take<f16_t>((size_t)z.mp * z.np * 2);
+    s.xt[0] = c.take<f16_t>((size_t)z.mp * z.np * 2);
+    s.xt[1] = c.take<f16_t>((size_t)z.mp * z.np * 2);
     s.a = c.take<f16_t>((size_t)z.mp * z.mp * 2);
     s.p = c.take<f16_t>((size_t)z.mp * z.mp * 2);
-    const int64_t tm = tiles_along(z.m, z.tile), tn = tiles_along(z.n, z.tile);
-    const int64_t sm = (z.m + kStage - 1) / kStage, sn = (z.n + kStage - 1) / kStage;
-    const int64_t gram = tm * (tm + 1) / 2, apply = tm * tn;
-    int64_t slots = gram + workgroups_for(z.tile, gram * sn);
-    if (gram + workgroups_for(z.tile, gram * sm) > slots) slots = gram + workgroups_for(z.tile, gram * sm);
-    if (apply + workgroups_for(z.tile, apply * sm) > slots) slots = apply + workgroups_for(z.tile, apply * sm);
-    s.parts = c.take<float>((size_t)slots * z.tile * z.tile);
+    size_t parts = 0;
+    for (const auto &of_terms : z.cut)
+        for (const Cut &cut : of_terms) {
+            const size_t need = (size_t)cut.slots * cut.tile * cut.tile;
+            if (need > parts) parts = need;
+        }
+    s.parts = c.take<float>(parts);
     s.norms = c.take<double>(kNormBlocks);
     s.bytes = c.used;
     return s;
 }
 
-cn_status product(const Product &g, int tile, int workgroups, int device, hipStream_t st) {
+template <int TILE, int TERMS, int FINISH>
+cn_status run_product(const Product &g, const Cut &c, int device, hipStream_t st) {
     static OncePerDevice configured;
-    if (configured.first(device)) {
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&product_kernel<256>), hipFuncAttributeMaxDynamicSharedMemorySize, 4 * 256 * 128));
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&product_kernel<128>), hipFuncAttributeMaxDynamicSharedMemorySize, 4 * 128 * 128));
-    }
-    if (tile == 256)
-        hipLaunchKernelGGL((product_kernel<256>), dim3(workgroups), dim3(threads_of<256>()), 4 * 256 * 128, st, g);
-    else
-        hipLaunchKernelGGL((product_kernel<128>), dim3(workgroups), dim3(threads_of<128>()), 4 * 128 * 128, st, g);
+    if (configured.first(device))
+        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&product_kernel<TILE, TERMS, FINISH>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   lds_of<TILE>()));
+    hipLaunchKernelGGL((product_kernel<TILE, TERMS, FINISH>), dim3(c.workgroups), dim3(threads_of<TILE>()), lds_of<TILE>(), st, g);
+    if (c.slots > 0)
+        hipLaunchKernelGGL((join_kernel<TILE, FINISH>), dim3((c.tiles - c.whole) * (TILE / 32) * (TILE / 32) / 4), dim3(256), 0, st, g, c.whole);
     CN_HIP(hipGetLastError());
     return CN_OK;
+}
+template <int FINISH>
+cn_status run_product(const Product &g, const Cut &c, int terms, int device, hipStream_t st) {
+    if (terms == 3 || FINISH == LAST)  // the last steps are always products of all parts
+        return c.tile == 256 ? run_product<256, 3, FINISH>(g, c, device, st) : c.tile == 128 ? run_product<128, 3, FINISH>(g, c, device, st)
+                                                                                             : run_product<64, 3, FINISH>(g, c, device, st);
+    if constexpr (FINISH != LAST)
+        return c.tile == 256 ? run_product<256, 1, FINISH>(g, c, device, st) : c.tile == 128 ? run_product<128, 1, FINISH>(g, c, device, st)
+                                                                                             : run_product<64, 1, FINISH>(g, c, device, st);
+    return CN_ERR_ARG;
 }
 
 struct Result {
@@ -500,47 +862,38 @@ cn_status newton_schulz(const Source &src, int steps, const Result &res, const S
     const int norm_blocks = (int)(norm_tiles < kNormBlocks ? norm_tiles : kNormBlocks);
     hipLaunchKernelGGL((norm_kernel<T>), dim3(norm_blocks), dim3(256), 0, st, src, s.norms);
     hipLaunchKernelGGL((split_kernel<T>), dim3((unsigned)((z.mp / 64) * (z.np / 64))), dim3(256), 0, st, src, s.norms, norm_blocks, z.flip,
-                       z.mp, z.np, s.x, s.xt);
+                       z.mp, z.np, s.x, s.xt[0]);
     CN_HIP(hipGetLastError());
-    const int tm = (int)tiles_along(z.m, z.tile), tn = (int)tiles_along(z.n, z.tile);
-    const int sm = (int)((z.m + kStage - 1) / kStage), sn = (int)((z.n + kStage - 1) / kStage);
-    const int gram_tiles = tm * (tm + 1) / 2, side = z.tile / 64;
+    int at = 0;  // which X^T is current
     for (int step = 0; step < steps; ++step) {
-        for (int which = 0; which < 3; ++which) {  // A = X X^T, A A, X^T P
+        for (int which = GRAM; which <= STEP; ++which) {
+            const bool full = res.dtype != CN_BF16 || step + 2 >= steps;
+            const Cut &c = z.cut[full][which];
             Product g{};
-            g.u = which == 0 ? s.x : which == 1 ? s.a : s.xt;
-            g.v = which == 0 ? s.x : which == 1 ? s.a : s.p;
-            g.u_cols = which == 0 ? z.np : z.mp;
+            g.u = which == GRAM ? s.x : which == POLY ? s.a : s.xt[at];
+            g.v = which == GRAM ? s.x : which == POLY ? s.a : s.p;
+            g.u_cols = which == GRAM ? z.np : z.mp;
             g.v_cols = g.u_cols;
-            g.tiles_j = tm;
-            g.symmetric = which != 2;
-            g.tiles = which == 2 ? tn * tm : gram_tiles;
-            g.stages = which == 0 ? sn : sm;
+            g.tiles_j = c.tiles_j;
+            g.stages = c.stages;
+            g.triangle = which != STEP;
+            for (int i = 0; i < kMaxGroups; ++i) g.group[i] = c.group[i];
             g.parts = s.parts;
-            const int64_t total = (int64_t)g.tiles * g.stages;
-            const int W = workgroups_for(z.tile, total);
-            cn_status status = product(g, z.tile, W, device, st);
+            g.old = which == POLY ? s.a : s.x;
+            g.to = which == GRAM ? s.a : which == POLY ? s.p : s.x;
+            g.to_cols = which == STEP ? z.np : z.mp;
+            g.to_t = s.xt[at ^ 1];
+            g.to_t_cols = z.mp;
+            g.out = res.out; g.out_dtype = res.dtype; g.ldo = res.ldo; g.m = z.m; g.n = z.n; g.flip = z.flip;
+            g.wide = res.ldo % 4 == 0 && aligned_to(res.out, 4 * dtype_bytes(res.dtype));
+            g.update = res.update; g.keep = res.keep; g.rate = res.rate;
+            const int terms = full ? 3 : 1;
+            const cn_status status = which == GRAM ? run_product<GRAM>(g, c, terms, device, st)
+                                   : which == POLY ? run_product<POLY>(g, c, terms, device, st)
+                                   : step + 1 < steps ? run_product<STEP>(g, c, terms, device, st) : run_product<LAST>(g, c, 3, device, st);
             if (status != CN_OK) return status;
-            FinishArgs f{};
-            f.parts = s.parts;
-            f.tile = z.tile; f.tiles_j = tm; f.symmetric = g.symmetric; f.stages = g.stages; f.workgroups = W;
-            f.total = total;
-            f.old = which == 1 ? s.a : s.xt;
-            f.cols = z.mp;
-            f.to = which == 0 ? s.a : which == 1 ? s.p : s.xt;
-            f.to_t = which == 0 ? s.a : which == 1 ? s.p : s.x;
-            f.cols_t = which == 2 ? z.np : z.mp;
-            f.out = res.out; f.ldo = res.ldo; f.m = z.m; f.n = z.n; f.flip = z.flip;
-            f.update = res.update; f.keep = res.keep; f.rate = res.rate;
-            const dim3 grid((unsigned)(g.tiles * side * side));
-            if (which == 0)             hipLaunchKernelGGL((finish_kernel<GRAM, float>), grid, dim3(256), 0, st, f);
-            else if (which == 1)        hipLaunchKernelGGL((finish_kernel<POLY, float>), grid, dim3(256), 0, st, f);
-            else if (step + 1 < steps)  hipLaunchKernelGGL((finish_kernel<STEP, float>), grid, dim3(256), 0, st, f);
-            else if (res.dtype == CN_F32) hipLaunchKernelGGL((finish_kernel<LAST, float>), grid, dim3(256), 0, st, f);
-            else if (res.dtype == CN_F16) hipLaunchKernelGGL((finish_kernel<LAST, f16_t>), grid, dim3(256), 0, st, f);
-            else                        hipLaunchKernelGGL((finish_kernel<LAST, bf16_t>), grid, dim3(256), 0, st, f);
-            CN_HIP(hipGetLastError());
         }
+        at ^= 1;
     }
     return CN_OK;
 }

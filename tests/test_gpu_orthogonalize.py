@@ -4,7 +4,9 @@ Tolerance.  A step maps singular values by p(s) = a s + b s^3 + c s^5; as a map 
 Frobenius norm is max |p'| on [0, 1.21], which is below 4.2.  An error of relative size e in each step is therefore at most
 e (4.2^5 - 1) / 3.2 = 408 e after five.  A step's own errors are roundings of 2^-24 (fp32 sums) and 2^-22 (the two-part operands) at a
 handful of places (A, A A, P, the product, the stored X), independent from element to element: e = 2^-21 covers eight of
-them.  So 408 * 2^-21 = 2e-4 of |out|_F, and for 16-bit results half a step of each element on top.  (One lost
+them.  So 408 * 2^-21 = 2e-4 of |out|_F, and for 16-bit results half a step of each element on top (for bfloat16, 2^-8, that is
+more than the 1e-3 its shorter products may cost: their roundings of 2^-12 in the first three steps pass through p of the
+last two, whose slope on the interval that they are in by then, 0.7 to 1.2, is what contracts them).  (One lost
 part of an operand is 2^-12 per product, and shows as 1e-3 to 3e-3.)"""
 import numpy as np
 import pytest
