@@ -32,6 +32,7 @@ typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTileN = 16, kTileK = 128;
+template <int N> struct Constant { static constexpr int value = N; };
 
 int64_t tiles_n_of(int64_t N) { return (N + kTileN - 1) / kTileN; }
 int64_t tiles_k_of(int64_t K) { return (K + kTileK - 1) / kTileK; }
@@ -45,7 +46,6 @@ struct GemmW4Args {
     void *out;
     int64_t M, N, K, lda, ldo;
     int tiles_k, tiles_n;
-    int group_shift;       // group = 1 << group_shift
     int vec_a;             // rows of A allow 16-byte loads
 };
 
@@ -71,19 +71,17 @@ template <> struct Kind<f16_t> {
     }
 };
 
-// Words of the B operand from eight codes: word j holds k = 2 j and 2 j + 1 of the lane, so nibbles 2 j and 2 j + 1.  They are
-// moved to the low and the high half: first the odd nibbles up by 12 bits (w << 12), then both to their place.
+// Operand words from eight codes: word j takes nibbles j and j + 4, which lie 16 bits apart: one shift and one and-or for two
+// weights.  So word j of the A operand has to hold the numbers j and j + 4 of the lane's eight as well; the sum over k does
+// not mind.  (In the order 2 j, 2 j + 1 a word takes five operations.)
 template <typename T>
 __device__ __forceinline__ u32x4 expand(uint32_t w) {
     using Q = Kind<T>;
     u32x4 b;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        // nibble 2 j from bit 8 j to bit kShift, nibble 2 j + 1 from bit 8 j + 4 to bit 16 + kShift
-        const int down = 8 * j - Q::kShift, up = 12 + Q::kShift - 8 * j;
-        const uint32_t lo = down >= 0 ? w >> down : w << -down;
-        const uint32_t hi = up >= 0 ? w << up : w >> -up;
-        b[j] = (lo & (Q::kMask & 0xffffu)) | (hi & (Q::kMask & 0xffff0000u)) | Q::kMagic;
+        const int down = 4 * j - Q::kShift;  // nibble j from bit 4 j to bit kShift
+        b[j] = ((down >= 0 ? w >> down : w << -down) & Q::kMask) | Q::kMagic;
     }
     return b;
 }
@@ -92,14 +90,16 @@ __device__ __forceinline__ u32x4 expand(uint32_t w) {
 template <typename T>
 __device__ __forceinline__ void operand(const u32x4 (&raw)[sizeof(T) / 2], u32x4 (&part)[Kind<T>::kParts]) {
     if constexpr (sizeof(T) == 2) {
-        part[0] = raw[0];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)  // halves j of the eight and j + 4
+            part[0][j] = __builtin_amdgcn_perm(raw[0][2 + (j >> 1)], raw[0][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             uint32_t piece[3][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const uint32_t x = raw[(2 * j + e) >> 2][(2 * j + e) & 3];
+                const uint32_t x = raw[e][j];
                 const uint32_t h = x & 0xffff0000u;  // the first eight bits
                 const float r = __uint_as_float(x) - __uint_as_float(h);
                 const uint32_t m = __float_as_uint(r) & 0xffff0000u;
@@ -109,16 +109,41 @@ __device__ __forceinline__ void operand(const u32x4 (&raw)[sizeof(T) / 2], u32x4
                 piece[2][e] = __float_as_uint(l);
             }
 #pragma unroll
-            for (int p = 0; p < 3; ++p) part[p][j] = (piece[p][0] >> 16) | (piece[p][1] & 0xffff0000u);
+            for (int p = 0; p < 3; ++p) part[p][j] = __builtin_amdgcn_perm(piece[p][1], piece[p][0], 0x07060302u);
         }
     }
 }
 
-// NT tiles of 16 columns and MB blocks of 16 rows per workgroup, WAVES wavefronts that split K.
-template <typename T, int NT, int MB, int WAVES>
+// Eight k of a row, from k on, as stored words; element by element: zeros past K.
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void load_eight(const T *row, int64_t k, int64_t K, u32x4 (&raw)[sizeof(T) / 2]) {
+    constexpr int kRaw = sizeof(T) / 2;
+    if (WHOLE) {
+#pragma unroll
+        for (int r = 0; r < kRaw; ++r) raw[r] = *(reinterpret_cast<const u32x4 *>(row + k) + r);
+        return;
+    }
+    uint32_t words[4 * kRaw];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t v = k + e < K ? (uint32_t)reinterpret_cast<const uint16_t *>(row)[k + e] : 0u;
+            words[e >> 1] = (e & 1) ? words[e >> 1] | v << 16 : v;
+        } else {
+            words[e] = k + e < K ? reinterpret_cast<const uint32_t *>(row)[k + e] : 0u;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kRaw; ++r) raw[r] = u32x4{words[4 * r], words[4 * r + 1], words[4 * r + 2], words[4 * r + 3]};
+}
+
+// NT tiles of 16 columns and MB blocks of 16 rows per workgroup, WAVES wavefronts that split K, GROUPS scales per 128 rows.
+// Codes and scales are requested kAhead tiles of 128 rows before they are used, A of a single block of rows one tile.
+template <typename T, int NT, int MB, int WAVES, int GROUPS>
 __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
     using Q = Kind<T>;
-    constexpr int kRaw = sizeof(T) / 2, kParts = Q::kParts;
+    constexpr int kRaw = sizeof(T) / 2, kParts = Q::kParts, kAhead = MB > 1 || (WAVES == 16 && sizeof(T) == 4) ? 1 : 2, kSpan = 4 / GROUPS;
+    constexpr bool kAheadA = MB == 1;
     extern __shared__ __attribute__((aligned(16))) float sums[];  // [WAVES][MB][NT][64][4]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int h = lane >> 4, c = lane & 15;
@@ -131,7 +156,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
 #pragma unroll
     for (int b = 0; b < MB; ++b) {  // rows past the last read the last: nothing of theirs is stored
         const int64_t m = m0 + b * 16 + c;
-        row[b] = (const T *)g.a + (m < g.M ? m : g.M - 1) * g.lda;
+        row[b] = (const T *)g.a + (m < g.M ? m : g.M - 1) * g.lda + 8 * h;
     }
     const u32x4 *codes[NT];
     int64_t column[NT];
@@ -142,6 +167,35 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
         const int64_t n = (int64_t)tn * kTileN + c;
         column[t] = n < g.N ? n : g.N - 1;
     }
+    const int last_group = (int)((g.K - 1) / (32 * kSpan));  // a group that lies wholly past K has no scale; its sums are zero
+
+    struct Slot {
+        u32x4 w[NT];
+        float scale[NT][GROUPS], zero[NT][GROUPS];
+    };
+    Slot slots[kAhead];
+    u32x4 ahead_a[2][kAheadA ? 4 : 1][kRaw];
+    const int64_t full = g.vec_a ? g.K / kTileK : 0;  // tiles of A that are read 16 bytes at a time; the others element by element
+    const int kw = __builtin_amdgcn_readfirstlane((int)(full < k0 ? k0 : full < k1 ? full : k1));
+    auto request = [&](Slot &s, int kb) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            s.w[t] = codes[t][(int64_t)kb * 64];
+#pragma unroll
+            for (int q = 0; q < GROUPS; ++q) {
+                const int group = kb * GROUPS + q < last_group ? kb * GROUPS + q : last_group;
+                const int64_t at = (int64_t)group * g.N + column[t];
+                s.scale[t][q] = g.scales[at];
+                s.zero[t][q] = g.zeros ? (float)g.zeros[at] : 8.0f;
+            }
+        }
+    };
+    auto request_a = [&](u32x4 (&a)[kAheadA ? 4 : 1][kRaw], int kb) {
+        if constexpr (kAheadA) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) load_eight<true>(row[0], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, a[q]);
+        }
+    };
 
     f32x4 total[MB][NT];
 #pragma unroll
@@ -150,61 +204,32 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
         for (int t = 0; t < NT; ++t) total[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     const u32x4 ones = {Q::kOnes, Q::kOnes, Q::kOnes, Q::kOnes};
 
-    u32x4 w[NT];
-    if (k0 < k1) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) w[t] = codes[t][(int64_t)k0 * 64];
-    }
-    for (int kb = k0; kb < k1; ++kb) {
-        u32x4 next[NT];
-        const int ahead = kb + 1 < k1 ? kb + 1 : kb;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) next[t] = codes[t][(int64_t)ahead * 64];
-        u32x4 raw[MB][4][kRaw];
-        const int64_t kk = (int64_t)kb * kTileK + 8 * h;
-        if (g.vec_a && (int64_t)kb * kTileK + kTileK <= g.K) {
-#pragma unroll
-            for (int b = 0; b < MB; ++b)
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int r = 0; r < kRaw; ++r) raw[b][s][r] = *(reinterpret_cast<const u32x4 *>(row[b] + kk + 32 * s) + r);
-        } else {  // element by element, zeros past K
-#pragma unroll
-            for (int b = 0; b < MB; ++b)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    uint32_t words[4 * kRaw];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int64_t k = kk + 32 * s + e;
-                        if constexpr (sizeof(T) == 2) {
-                            const uint32_t v = k < g.K ? (uint32_t)reinterpret_cast<const uint16_t *>(row[b])[k] : 0u;
-                            words[e >> 1] = (e & 1) ? words[e >> 1] | v << 16 : v;
-                        } else {
-                            words[e] = k < g.K ? reinterpret_cast<const uint32_t *>(row[b])[k] : 0u;
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < kRaw; ++r) raw[b][s][r] = u32x4{words[4 * r], words[4 * r + 1], words[4 * r + 2], words[4 * r + 3]};
-                }
-        }
+    auto consume = [&](const Slot &s, const u32x4 (&a)[kAheadA ? 4 : 1][kRaw], int kb, auto whole) {
+        constexpr bool kWhole = decltype(whole)::value != 0;
         f32x4 acc[MB][NT], sum_a[MB];
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
-            sum_a[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < 4; ++q) {
+            if (q % kSpan == 0) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+                for (int b = 0; b < MB; ++b) {
+                    sum_a[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+                    for (int t = 0; t < NT; ++t) acc[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
             u32x4 bw[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) bw[t] = expand<T>(w[t][s]);
+            for (int t = 0; t < NT; ++t) bw[t] = expand<T>(s.w[t][q]);
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
-                u32x4 part[kParts];
-                operand<T>(raw[b][s], part);
+                u32x4 raw[kRaw], part[kParts];
+                if constexpr (kAheadA && kWhole) {
+#pragma unroll
+                    for (int r = 0; r < kRaw; ++r) raw[r] = a[q][r];
+                } else {
+                    load_eight<kWhole>(row[b], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, raw);
+                }
+                operand<T>(raw, part);
 #pragma unroll
                 for (int p = kParts - 1; p >= 0; --p) {
                     sum_a[b] = Q::mfma(part[p], ones, sum_a[b]);
@@ -212,30 +237,39 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
                     for (int t = 0; t < NT; ++t) acc[b][t] = Q::mfma(part[p], bw[t], acc[b][t]);
                 }
             }
-            if (((s + 1) << 5 & ((1 << g.group_shift) - 1)) == 0) {  // the end of a group
-                // a group that lies wholly past K has no scale; its sums are zero
-                int64_t group = ((int64_t)kb * kTileK + 32 * s) >> g.group_shift;
-                const int64_t last = (g.K - 1) >> g.group_shift;
-                group = group < last ? group : last;
+            if (q % kSpan == kSpan - 1) {  // the end of a group
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const int64_t at = group * g.N + column[t];
-                    const float scale = g.scales[at];
-                    const float offset = 16.0f + (g.zeros ? (float)g.zeros[at] : 8.0f);
+                    const float scale = s.scale[t][q / kSpan], offset = 16.0f + s.zero[t][q / kSpan];
 #pragma unroll
                     for (int b = 0; b < MB; ++b)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            total[b][t][r] += scale * (acc[b][t][r] - offset * sum_a[b][r]);
-                            acc[b][t][r] = 0.0f;
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            total[b][t][r] = __builtin_fmaf(scale, __builtin_fmaf(-offset, sum_a[b][r], acc[b][t][r]), total[b][t][r]);
                 }
-#pragma unroll
-                for (int b = 0; b < MB; ++b) sum_a[b] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
         }
+    };
+    // a request past the last tile reads the last again (unused)
+    auto last = [&](int kb) { return kb < kw ? kb : kw - 1; };
+    if (k0 < kw) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) w[t] = next[t];
+        for (int d = 0; d < kAhead; ++d) request(slots[d], last(k0 + d));
+        request_a(ahead_a[0], k0);
+    }
+    for (int kb = k0; kb < kw; kb += kAhead) {
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) {
+            if (kb + d >= kw) break;
+            request_a(ahead_a[(d + 1) & 1], last(kb + d + 1));
+            consume(slots[d], ahead_a[d & 1], kb + d, Constant<1>{});
+            request(slots[d], last(kb + d + kAhead));
+        }
+    }
+#pragma unroll 1
+    for (int kb = kw; kb < k1; ++kb) {
+        request(slots[0], kb);
+        consume(slots[0], ahead_a[0], kb, Constant<0>{});
     }
 
     // Lane (h, c) holds rows 4 h .. 4 h + 3 of column c of each block.
@@ -257,139 +291,197 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
     }
 }
 
-template <typename T, int NT, int MB, int WAVES>
-cn_status launch_gemm(const GemmW4Args &g, int device, hipStream_t st) {
-    const size_t lds = (size_t)WAVES * MB * NT * 256 * sizeof(float);
-    static OncePerDevice configured;
-    if (lds > 65536 && configured.first(device))
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&gemm_w4_kernel<T, NT, MB, WAVES>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+template <typename T, int NT, int MB, int WAVES, int GROUPS>
+cn_status launch_gemm(const GemmW4Args &g, hipStream_t st) {
+    constexpr size_t lds = (size_t)WAVES * MB * NT * 256 * sizeof(float);
+    static_assert(lds <= 65536, "no more than a launch may ask for by itself");
     const dim3 grid((unsigned)((g.tiles_n + NT - 1) / NT), (unsigned)((g.M + 16 * MB - 1) / (16 * MB)));
-    hipLaunchKernelGGL((gemm_w4_kernel<T, NT, MB, WAVES>), grid, dim3(WAVES * 64), lds, st, g);
+    hipLaunchKernelGGL((gemm_w4_kernel<T, NT, MB, WAVES, GROUPS>), grid, dim3(WAVES * 64), lds, st, g);
     CN_HIP(hipGetLastError());
     return CN_OK;
 }
 
-template <typename T>
-cn_status run_gemm(const GemmW4Args &g, int device, hipStream_t st) {
-    if (g.M > 16) return g.M > 32 ? launch_gemm<T, 2, 4, 8>(g, device, st) : launch_gemm<T, 2, 2, 8>(g, device, st);
-    // wide workgroups read A less often, narrow ones are enough to fill the chip
-    if (g.tiles_n >= 2048) return launch_gemm<T, 4, 1, 8>(g, device, st);
-    if (g.tiles_n >= 1024) return launch_gemm<T, 2, 1, 8>(g, device, st);
-    return launch_gemm<T, 1, 1, 8>(g, device, st);
+template <typename T, int GROUPS>
+cn_status run_gemm(const GemmW4Args &g, hipStream_t st) {
+    if (g.M > 32) return launch_gemm<T, GROUPS == 4 ? 1 : 2, 4, 8, GROUPS>(g, st);  // (two columns of groups of 32 would spill)
+    if (g.M > 16) return launch_gemm<T, 2, 2, 8, GROUPS>(g, st);
+    // Wide workgroups share A and its sums (one row of 16384 x 16384: 33.0 us, 38.3 us with narrow ones, 34.5 with four tiles of
+    // columns, 34.0 with one tile of 128 rows ahead, 38.6 with four); narrow ones, with K among more wavefronts, fill the chip.
+    if (g.tiles_n >= 512) return launch_gemm<T, 2, 1, 8, GROUPS>(g, st);
+    if (g.tiles_n > 256) return launch_gemm<T, 1, 1, 8, GROUPS>(g, st);
+    return launch_gemm<T, 1, 1, 16, GROUPS>(g, st);
 }
 
 // ---- quantisation --------------------------------------------------------------------------------------------------------
-// A workgroup takes 128 rows of 64 columns, lane (h, column) rows 32 t + 8 h + i: the codes of its four words.
+// A workgroup takes 128 rows of 64 C columns, lane (h, l) rows 32 t + 8 h + i of C neighbouring ones: the codes of its four words
+// each.  Workgroups that follow each other are neighbours along the rows of W.  (16384 x 8192 bf16, with workgroups going down
+// the columns, one column a lane and every lane finding the scales by itself: 300 us.)
 struct QuantArgs {
     int64_t K, N, ldw;
-    int64_t tiles_k, tiles_n;
+    int64_t tiles_k, tiles_n, blocks_n;
     int group;
 };
+constexpr float kLargest = 3.402823466e38f;
 
-template <typename T, bool ZP>
+// Eight codes, decided exactly: the remainder of a candidate has a single rounding that keeps its comparison with scale / 2 (it is a
+// multiple of scale's last place no larger than scale).  A scale of 0 or NaN gives the code that stands for 0.
+template <int C>
+__device__ __forceinline__ uint32_t exact_codes(const float (&v)[8][C], int j, float scale, float zero) {
+    const float lift = scale < 0x1p-90f ? 0x1p90f : 1.0f;  // keeps the reciprocal finite; exact either way
+    const float s = scale * lift, inverse = scale > 0.0f ? 1.0f / s : 0.0f;
+    uint32_t packed = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = v[i][j] * lift;
+        float q = rintf(x * inverse);
+        const float rest = __builtin_fmaf(-q, s, x), twice = rest + rest;
+        if (twice > s || (twice == s && ((int)q & 1))) q += 1.0f;
+        else if (-twice > s || (-twice == s && ((int)q & 1))) q -= 1.0f;
+        q = fminf(fmaxf(q + zero, 0.0f), 15.0f);
+        packed |= (inverse > 0.0f ? (uint32_t)q : (uint32_t)zero) << (4 * i);
+    }
+    return packed;
+}
+
+template <typename T, bool ZP, int C>
 __global__ __launch_bounds__(256) void quantize_kernel(QuantArgs g, const T *__restrict__ w, u32x4 *__restrict__ codes,
                                                        float *__restrict__ scales, uint8_t *__restrict__ zeros) {
-    __shared__ float top[4][4][64], low[4][4][64];  // [t][h][column]: largest value (magnitude), smallest
-    const int h = threadIdx.x >> 6, col = threadIdx.x & 63;
-    const int64_t kb = blockIdx.x % g.tiles_k, n = blockIdx.x / g.tiles_k * 64 + col;
+    constexpr int kCols = 64 * C;
+    __shared__ float top[4][4][kCols], low[ZP ? 4 : 1][4][kCols];  // [t][h][column]: largest value (magnitude), smallest
+    __shared__ float scale_of[4][kCols], zero_of[4][kCols];        // [group of the 128 rows][column]
+    const int h = threadIdx.x >> 6, l = threadIdx.x & 63;
+    const int64_t kb = blockIdx.x / g.blocks_n, n0 = blockIdx.x % g.blocks_n * kCols, n = n0 + l * C;
     const int64_t k0 = kb * kTileK + 8 * h;
-    float v[4][8];
+    const bool inside = kb * kTileK + kTileK <= g.K && n0 + kCols <= g.N;  // of the whole workgroup
+    float v[4][8][C];
+    if (inside) {
+        const T *at = w + k0 * g.ldw + n;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) load_f32<C>(at + (32 * t + i) * g.ldw, v[t][i]);
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t k = k0 + 32 * t + i;
+                if (k < g.K && n < g.N) {
+                    load_f32<C>(w + k * g.ldw + n, v[t][i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < C; ++j) v[t][i][j] = 0.0f;  // zero changes no range: it belongs to every one
+                }
+            }
+    }
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int64_t k = k0 + 32 * t + i;
-            v[t][i] = k < g.K && n < g.N ? (float)w[k * g.ldw + n] : 0.0f;  // zero changes no range: it belongs to every one
-        }
+        for (int j = 0; j < C; ++j) {
+            float hi = 0.0f, lo = 0.0f, odd = 0.0f;  // odd: NaN if something is not finite
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        float hi = 0.0f, lo = 0.0f;
-        bool odd = false;  // something is not finite
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            odd |= !(fabsf(v[t][i]) <= 3.402823466e38f);
-            if (ZP) {
-                hi = fmaxf(hi, v[t][i]);
-                lo = fminf(lo, v[t][i]);
-            } else {
-                hi = fmaxf(hi, fabsf(v[t][i]));
+            for (int i = 0; i < 8; ++i) {
+                const float x = v[t][i][j];
+                odd = __builtin_fmaf(x, 0.0f, odd);
+                hi = fmaxf(hi, ZP ? x : fabsf(x));
+                if (ZP) lo = fminf(lo, x);
             }
+            top[t][h][l * C + j] = odd == 0.0f ? hi : __uint_as_float(0x7f800000u);
+            if (ZP) low[t][h][l * C + j] = lo;
         }
-        top[t][h][col] = odd ? __uint_as_float(0x7f800000u) : hi;
-        if (ZP) low[t][h][col] = lo;
+    __syncthreads();
+    const int span = g.group / 32, groups = 4 / span;  // words of t per group: 1, 2 or 4
+    for (int x = threadIdx.x; x < groups * kCols; x += 256) {
+        const int group = x / kCols, col = x % kCols;
+        float hi = 0.0f, lo = 0.0f;
+        for (int t = group * span; t < group * span + span; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                hi = fmaxf(hi, top[t][q][col]);
+                if (ZP) lo = fminf(lo, low[t][q][col]);
+            }
+        const bool finite = hi <= kLargest;
+        // one rounding to fp32: quotients by 7 and 15 are never so near a midpoint that the one to 64 bits matters
+        float scale = (float)(((double)hi - (double)lo) / (ZP ? 15.0 : 7.0));
+        float zero = ZP ? (scale > 0.0f && finite ? (float)rint(-(double)lo / (double)scale) : 0.0f) : 8.0f;
+        zero = fminf(fmaxf(zero, 0.0f), 15.0f);
+        if (!finite) scale = __uint_as_float(0x7fc00000u);  // the whole group decodes to NaN
+        scale_of[group][col] = scale;
+        zero_of[group][col] = zero;
+        const int64_t at = kb * groups + group;
+        if (n0 + col < g.N && at * g.group < g.K) {
+            scales[at * g.N + n0 + col] = scale;
+            if (ZP) zeros[at * g.N + n0 + col] = (uint8_t)zero;
+        }
     }
     __syncthreads();
-    u32x4 word;
-    float scale = 0.0f, inverse = 0.0f, lift = 1.0f, zero = 8.0f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int span = g.group / 32;  // words of t per group: 1, 2 or 4
-        if (t % span == 0) {
-            float hi = 0.0f, lo = 0.0f;
-            for (int s = t; s < t + span; ++s)
+    for (int j = 0; j < C; ++j) {
+        u32x4 word;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    hi = fmaxf(hi, top[s][q][col]);
-                    if (ZP) lo = fminf(lo, low[s][q][col]);
-                }
-            const bool finite = hi <= 3.402823466e38f;
-            // one rounding to fp32: quotients by 7 and 15 are never so near a midpoint that the one to 64 bits matters
-            scale = (float)(((double)hi - (double)lo) / (ZP ? 15.0 : 7.0));
-            zero = ZP ? (scale > 0.0f && finite ? (float)rint(-(double)lo / (double)scale) : 0.0f) : 8.0f;
-            zero = fminf(fmaxf(zero, 0.0f), 15.0f);
-            if (!finite) scale = __uint_as_float(0x7fc00000u);  // the whole group decodes to NaN
-            lift = scale < 0x1p-90f ? 0x1p90f : 1.0f;  // keeps the reciprocal finite; exact either way
-            inverse = scale > 0.0f ? 1.0f / (scale * lift) : 0.0f;
-            const int64_t group = (kb * kTileK + 32 * t) / g.group;
-            if (h == 0 && n < g.N && group * g.group < g.K) {
-                scales[group * g.N + n] = scale;
-                if (ZP) zeros[group * g.N + n] = (uint8_t)zero;
+        for (int t = 0; t < 4; ++t) {
+            const float scale = scale_of[t / span][l * C + j], zero = zero_of[t / span][l * C + j];
+            // round(v / scale), ties to even.  Nearly always the product with the reciprocal settles it (off by 10^-6 at most);
+            // where one of eight comes near a half, or the scale is tiny, all eight are decided exactly.
+            const float direct = scale > 0x1p-90f ? 1.0f / scale : 0.0f;
+            uint32_t packed = 0u;
+            float far = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = v[t][i][j] * direct, q = rintf(f);
+                far = fmaxf(far, fabsf(f - q));
+                packed |= (uint32_t)fminf(fmaxf(q + zero, 0.0f), 15.0f) << (4 * i);
             }
+            if (!(far < 0.49999f && direct > 0.0f)) packed = exact_codes<C>(v[t], j, scale, zero);
+            if (!inside) {
+                const int64_t rows = g.K - (k0 + 32 * t);  // that there are
+                if (n + j >= g.N || rows <= 0) packed = 0u;
+                else if (rows < 8) packed &= (1u << (4 * rows)) - 1u;
+            }
+            word[t] = packed;
         }
-        uint32_t packed = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            // round(v / scale), ties to even, decided exactly: the remainder of the candidate has a single rounding that keeps its
-            // comparison with scale / 2 (it is a multiple of scale's last place no larger than scale)
-            const float x = v[t][i] * lift, s = scale * lift;
-            float q = rintf(x * inverse);
-            const float rest = __builtin_fmaf(-q, s, x), twice = rest + rest;
-            if (twice > s || (twice == s && ((int)q & 1))) q += 1.0f;
-            else if (-twice > s || (-twice == s && ((int)q & 1))) q -= 1.0f;
-            q = fminf(fmaxf(q + zero, 0.0f), 15.0f);
-            const int64_t k = k0 + 32 * t + i;
-            const uint32_t code = inverse > 0.0f ? (uint32_t)q : (uint32_t)zero;
-            packed |= (k < g.K && n < g.N ? code : 0u) << (4 * i);
-        }
-        word[t] = packed;
+        const int64_t a = (n + j) / kTileN;
+        if (a < g.tiles_n) codes[(a * g.tiles_k + kb) * 64 + h * 16 + ((n + j) & 15)] = word;
     }
-    const int64_t a = n / kTileN;
-    if (a < g.tiles_n) codes[(a * g.tiles_k + kb) * 64 + h * 16 + (col & 15)] = word;
 }
 
-template <typename T, bool ZP>
+template <typename T, bool ZP, int C>
 __global__ __launch_bounds__(256) void dequantize_kernel(QuantArgs g, const u32x4 *__restrict__ codes, const float *__restrict__ scales,
                                                          const uint8_t *__restrict__ zeros, T *__restrict__ out) {
-    const int h = threadIdx.x >> 6, col = threadIdx.x & 63;
-    const int64_t kb = blockIdx.x % g.tiles_k, n = blockIdx.x / g.tiles_k * 64 + col;
+    const int h = threadIdx.x >> 6, l = threadIdx.x & 63;
+    const int64_t kb = blockIdx.x / g.blocks_n, n = blockIdx.x % g.blocks_n * (64 * C) + l * C;
     if (n >= g.N) return;
-    const u32x4 word = codes[(n / kTileN * g.tiles_k + kb) * 64 + h * 16 + (col & 15)];
+    u32x4 word[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) word[j] = codes[((n + j) / kTileN * g.tiles_k + kb) * 64 + h * 16 + ((n + j) & 15)];
     const int64_t k0 = kb * kTileK + 8 * h;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         const int64_t first = kb * kTileK + 32 * t;
         if (first >= g.K) break;
         const int64_t at = first / g.group * g.N + n;
-        const float scale = scales[at], zero = ZP ? (float)zeros[at] : 8.0f;
+        float scale[C], zero[C];
+        load_f32<C>(scales + at, scale);
+#pragma unroll
+        for (int j = 0; j < C; ++j) zero[j] = ZP ? (float)zeros[at + j] : 8.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int64_t k = k0 + 32 * t + i;
-            float v = ((float)((word[t] >> (4 * i)) & 15u) - zero) * scale;
-            asm volatile("" : "+v"(v));  // a product that becomes fp16 at once would skip its rounding to fp32
-            if (k < g.K) out[k * g.ldw + n] = (T)v;
+            float v[C];
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                v[j] = ((float)((word[j][t] >> (4 * i)) & 15u) - zero[j]) * scale[j];
+                asm volatile("" : "+v"(v[j]));  // a product that becomes fp16 at once would skip its rounding to fp32
+            }
+            if (k < g.K) store_f32<C>(out + k * g.ldw + n, v);
         }
     }
+}
+
+// Columns of a lane: two where their loads are whole words.
+QuantArgs quant_args(int64_t K, int64_t N, int64_t ld, int group, int columns) {
+    const int64_t wide = 64 * columns;
+    return QuantArgs{K, N, ld, tiles_k_of(K), tiles_n_of(N), (N + wide - 1) / wide, group};
 }
 
 cn_status check_weights(const char *what, int64_t K, int64_t N, int group) {
@@ -427,14 +519,19 @@ cn_status cn_quantize_4bit(const void *W, int dtype, int64_t K, int64_t N, int64
     Context *ctx;
     s = current_context(&ctx);
     if (s != CN_OK) return s;
-    const QuantArgs g{K, N, ldw, tiles_k_of(K), tiles_n_of(N), group};
-    const dim3 grid((unsigned)(g.tiles_k * ((N + 63) / 64)));
-    auto go = [&](auto zero) {
+    hipStream_t st = (hipStream_t)stream;
+    auto go = [&](auto zero, auto columns) {
         typedef decltype(zero) T;
-        if (zeros) hipLaunchKernelGGL((quantize_kernel<T, true>), grid, dim3(256), 0, (hipStream_t)stream, g, (const T *)W, (u32x4 *)codes, scales, zeros);
-        else       hipLaunchKernelGGL((quantize_kernel<T, false>), grid, dim3(256), 0, (hipStream_t)stream, g, (const T *)W, (u32x4 *)codes, scales, zeros);
+        constexpr int C = decltype(columns)::value;
+        const QuantArgs g = quant_args(K, N, ldw, group, C);
+        const dim3 grid((unsigned)(g.tiles_k * g.blocks_n));
+        if (zeros) hipLaunchKernelGGL((quantize_kernel<T, true, C>), grid, dim3(256), 0, st, g, (const T *)W, (u32x4 *)codes, scales, zeros);
+        else       hipLaunchKernelGGL((quantize_kernel<T, false, C>), grid, dim3(256), 0, st, g, (const T *)W, (u32x4 *)codes, scales, zeros);
     };
-    if (dtype == CN_F32) go(0.0f); else if (dtype == CN_F16) go((f16_t)0); else go((bf16_t)0);
+    const bool pairs = N % 2 == 0 && ldw % 2 == 0 && aligned_to(W, 2 * dtype_bytes(dtype));
+    if (dtype == CN_F32) go(0.0f, Constant<1>{});
+    else if (dtype == CN_F16) pairs ? go((f16_t)0, Constant<2>{}) : go((f16_t)0, Constant<1>{});
+    else pairs ? go((bf16_t)0, Constant<2>{}) : go((bf16_t)0, Constant<1>{});
     CN_HIP(hipGetLastError());
     return CN_OK;
 }
@@ -451,14 +548,19 @@ cn_status cn_dequantize_4bit(const int32_t *codes, const float *scales, const ui
     Context *ctx;
     s = current_context(&ctx);
     if (s != CN_OK) return s;
-    const QuantArgs g{K, N, ldo, tiles_k_of(K), tiles_n_of(N), group};
-    const dim3 grid((unsigned)(g.tiles_k * ((N + 63) / 64)));
-    auto go = [&](auto zero) {
+    hipStream_t st = (hipStream_t)stream;
+    auto go = [&](auto zero, auto columns) {
         typedef decltype(zero) T;
-        if (zeros) hipLaunchKernelGGL((dequantize_kernel<T, true>), grid, dim3(256), 0, (hipStream_t)stream, g, (const u32x4 *)codes, scales, zeros, (T *)out);
-        else       hipLaunchKernelGGL((dequantize_kernel<T, false>), grid, dim3(256), 0, (hipStream_t)stream, g, (const u32x4 *)codes, scales, zeros, (T *)out);
+        constexpr int C = decltype(columns)::value;
+        const QuantArgs g = quant_args(K, N, ldo, group, C);
+        const dim3 grid((unsigned)(g.tiles_k * g.blocks_n));
+        if (zeros) hipLaunchKernelGGL((dequantize_kernel<T, true, C>), grid, dim3(256), 0, st, g, (const u32x4 *)codes, scales, zeros, (T *)out);
+        else       hipLaunchKernelGGL((dequantize_kernel<T, false, C>), grid, dim3(256), 0, st, g, (const u32x4 *)codes, scales, zeros, (T *)out);
     };
-    if (dtype == CN_F32) go(0.0f); else if (dtype == CN_F16) go((f16_t)0); else go((bf16_t)0);
+    const bool pairs = N % 2 == 0 && ldo % 2 == 0 && aligned_to(out, 2 * dtype_bytes(dtype)) && aligned_to(scales, 8);
+    if (dtype == CN_F32) pairs ? go(0.0f, Constant<2>{}) : go(0.0f, Constant<1>{});
+    else if (dtype == CN_F16) pairs ? go((f16_t)0, Constant<2>{}) : go((f16_t)0, Constant<1>{});
+    else pairs ? go((bf16_t)0, Constant<2>{}) : go((bf16_t)0, Constant<1>{});
     CN_HIP(hipGetLastError());
     return CN_OK;
 }
@@ -481,12 +583,13 @@ cn_status cn_gemm_w4(int64_t M, int64_t N, int64_t K, const void *A, int dtype, 
     g.a = A; g.codes = (const u32x4 *)codes; g.scales = scales; g.zeros = zeros; g.out = out;
     g.M = M; g.N = N; g.K = K; g.lda = lda; g.ldo = ldo;
     g.tiles_k = (int)tiles_k_of(K); g.tiles_n = (int)tiles_n_of(N);
-    g.group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
     g.vec_a = aligned_to(A, 16) && lda % (16 / (int64_t)dtype_bytes(dtype)) == 0;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == CN_F32) return run_gemm<float>(g, ctx->device, st);
-    if (dtype == CN_F16) return run_gemm<f16_t>(g, ctx->device, st);
-    return run_gemm<bf16_t>(g, ctx->device, st);
+    auto go = [&](auto zero) -> cn_status {
+        typedef decltype(zero) T;
+        return group == 128 ? run_gemm<T, 1>(g, st) : group == 64 ? run_gemm<T, 2>(g, st) : run_gemm<T, 4>(g, st);
+    };
+    return dtype == CN_F32 ? go(0.0f) : dtype == CN_F16 ? go((f16_t)0) : go((bf16_t)0);
 }
 
 }  // extern "C"
