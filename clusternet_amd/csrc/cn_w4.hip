@@ -257,13 +257,14 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
         for (int d = 0; d < kAhead; ++d) request(slots[d], last(k0 + d));
         request_a(ahead_a[0], k0);
     }
-    for (int kb = k0; kb < kw; kb += kAhead) {
+    constexpr int kTurn = kAhead < 2 ? 2 : kAhead;  // the two buffers of A take turns
+    for (int kb = k0; kb < kw; kb += kTurn) {
 #pragma unroll
-        for (int d = 0; d < kAhead; ++d) {
+        for (int d = 0; d < kTurn; ++d) {
             if (kb + d >= kw) break;
             request_a(ahead_a[(d + 1) & 1], last(kb + d + 1));
-            consume(slots[d], ahead_a[d & 1], kb + d, Constant<1>{});
-            request(slots[d], last(kb + d + kAhead));
+            consume(slots[d % kAhead], ahead_a[d & 1], kb + d, Constant<1>{});
+            request(slots[d % kAhead], last(kb + d + kAhead));
         }
     }
 #pragma unroll 1
