@@ -116,9 +116,9 @@ __device__ __forceinline__ void operand(const u32x4 (&raw)[sizeof(T) / 2], u32x4
 
 // Eight k of a row, from k on, as stored words; element by element: zeros past K.
 template <bool WHOLE, typename T>
-__device__ __forceinline__ void load_eight(const T *row, int64_t k, int64_t K, u32x4 (&raw)[sizeof(T) / 2]) {
+__device__ __forceinline__ void load_eight(const T *row, int64_t k, int64_t K, bool vec, u32x4 (&raw)[sizeof(T) / 2]) {
     constexpr int kRaw = sizeof(T) / 2;
-    if (WHOLE) {
+    if (WHOLE || (vec && k + 8 <= K)) {
 #pragma unroll
         for (int r = 0; r < kRaw; ++r) raw[r] = *(reinterpret_cast<const u32x4 *>(row + k) + r);
         return;
@@ -142,7 +142,7 @@ __device__ __forceinline__ void load_eight(const T *row, int64_t k, int64_t K, u
 template <typename T, int NT, int MB, int WAVES, int GROUPS>
 __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
     using Q = Kind<T>;
-    constexpr int kRaw = sizeof(T) / 2, kParts = Q::kParts, kAhead = MB > 1 || (WAVES == 16 && sizeof(T) == 4) ? 1 : 2, kSpan = 4 / GROUPS;
+    constexpr int kRaw = sizeof(T) / 2, kParts = Q::kParts, kAhead = MB > 1 ? 1 : 2, kSpan = 4 / GROUPS;
     constexpr bool kAheadA = MB == 1;
     extern __shared__ __attribute__((aligned(16))) float sums[];  // [WAVES][MB][NT][64][4]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
     auto request_a = [&](u32x4 (&a)[kAheadA ? 4 : 1][kRaw], int kb) {
         if constexpr (kAheadA) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) load_eight<true>(row[0], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, a[q]);
+            for (int q = 0; q < 4; ++q) load_eight<true>(row[0], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, true, a[q]);
         }
     };
 
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
 #pragma unroll
                     for (int r = 0; r < kRaw; ++r) raw[r] = a[q][r];
                 } else {
-                    load_eight<kWhole>(row[b], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, raw);
+                    load_eight<kWhole>(row[b], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, g.vec_a != 0, raw);
                 }
                 operand<T>(raw, part);
 #pragma unroll
@@ -310,7 +310,7 @@ cn_status run_gemm(const GemmW4Args &g, hipStream_t st) {
     // columns, 34.0 with one tile of 128 rows ahead, 38.6 with four); narrow ones, with K among more wavefronts, fill the chip.
     if (g.tiles_n >= 512) return launch_gemm<T, 2, 1, 8, GROUPS>(g, st);
     if (g.tiles_n > 256) return launch_gemm<T, 1, 1, 8, GROUPS>(g, st);
-    return launch_gemm<T, 1, 1, 16, GROUPS>(g, st);
+    return launch_gemm<T, 1, 1, sizeof(T) == 2 ? 16 : 8, GROUPS>(g, st);  // (fp32 operands take too many registers for sixteen)
 }
 
 // ---- quantisation --------------------------------------------------------------------------------------------------------
