@@ -29,17 +29,18 @@ __device__ __forceinline__ void load_f32(const T *p, float (&v)[N]) {
         for (int i = 0; i < N; ++i) v[i] = (float)w[i];
     }
 }
-// fp32 to N consecutive elements, each rounded to nearest even once.
-template <int N, typename T>
+// fp32 to N consecutive elements, each rounded to nearest even once.  STREAM: past the caches, for what is not read again soon.
+template <int N, bool STREAM = false, typename T>
 __device__ __forceinline__ void store_f32(T *p, const float (&v)[N]) {
+    typename Pack<T, N>::type w;
     if constexpr (N == 1) {
-        *p = (T)v[0];
+        w = (T)v[0];
     } else {
-        typename Pack<T, N>::type w;
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = (T)v[i];
-        *reinterpret_cast<typename Pack<T, N>::type *>(p) = w;
     }
+    if constexpr (STREAM && N > 1) __builtin_nontemporal_store(w, reinterpret_cast<typename Pack<T, N>::type *>(p));
+    else *reinterpret_cast<typename Pack<T, N>::type *>(p) = w;
 }
 
 inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

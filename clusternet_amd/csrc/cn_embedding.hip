@@ -7,8 +7,8 @@
 // Gradient    dE[v] = scale * sum over {t : tok[t] = v} of dY[t], in fp32.
 //   1. The positions are sorted by token, stably, by a radix sort of my own digits: ceil(log2(rows + 1)) bits in as many
 //      passes as digits of at most kMaxDigit bits need (two for a table of up to 2^18 rows).  A token outside the table
-//      takes the key `rows` and so comes last.  Up to kBlockItems positions one workgroup does all passes in LDS; beyond,
-//      a pass is three launches (count digits per block, prefix sums per digit over the blocks, scatter).
+//      takes the key `rows` and so comes last.  Up to kSmallItems positions one workgroup does all passes in LDS; beyond,
+//      a pass is two or three launches (count digits per block, for many blocks prefix sums per digit, scatter).
 //   2. The sorted list is cut into chunks of equal length, so a token that makes up a large share of the text costs no more
 //      than any other.  A group of lanes walks its chunk, adds the rows of dY in sorted order and writes each run of one
 //      token as it ends.  A run that crosses a chunk's border leaves its part in the workspace instead.
@@ -24,8 +24,13 @@ namespace {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kSortRounds = 8;                                // items per lane
-constexpr int kBlockItems = kSortThreads * kSortRounds;       // items of one workgroup: 8192
+constexpr int kSmallRounds = 8;                               // items per lane of the sort in one workgroup, at most
+constexpr int kSmallItems = kSortThreads * kSmallRounds;      // 8192
+// Of the sort over many workgroups: a lane's items are ranked one after the other, so few of them and more workgroups (eight
+// a lane and 8 workgroups for 65536 tokens: 15 us a scatter).
+constexpr int kManyRounds = 2;
+constexpr int kManyItems = kSortThreads * kManyRounds;
+constexpr int kDirectBlocks = 64;  // up to so many, a workgroup adds up the counts of the others by itself: a launch less a pass
 constexpr int kMaxDigit = 9;                                  // bits of a digit
 constexpr int kMaxBins = 1 << kMaxDigit;
 
@@ -61,7 +66,8 @@ __global__ __launch_bounds__(256) void embedding_kernel(const T *__restrict__ ta
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[j][e] *= scale;
         }
-        store_f32<VEC>(out + t * ldo + col, v[j]);
+        // past the caches, which then hold the table's frequent rows (65536 x 2048 bf16: 59 us instead of 91)
+        store_f32<VEC, true>(out + t * ldo + col, v[j]);
     }
 }
 
@@ -76,16 +82,17 @@ __device__ __forceinline__ uint64_t lanes_alike(uint32_t digit, int bits, bool l
     return mask;
 }
 
-// Ranks the workgroup's items stably by digit.  In: digit[r] of item wave * 512 + r * 64 + lane (live[r]: it exists).
+// Ranks the workgroup's items stably by digit.  In: digit[r] of item (wave * R + r) * 64 + lane (live[r]: it exists).
 // Out: rank[r] = number of the workgroup's items of the same digit that come before it; counts[w][d] = exclusive prefix over
 // the wavefronts, totals[d] = the workgroup's items of digit d.
-__device__ __forceinline__ void rank_items(const uint32_t (&digit)[kSortRounds], const bool (&live)[kSortRounds], int bits,
-                                           uint32_t (*counts)[kMaxBins], uint32_t *totals, uint32_t (&rank)[kSortRounds]) {
+template <int R>
+__device__ __forceinline__ void rank_items(const uint32_t (&digit)[R], const bool (&live)[R], int bits,
+                                           uint32_t (*counts)[kMaxBins], uint32_t *totals, uint32_t (&rank)[R]) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, bins = 1 << bits;
     for (int i = tid; i < kSortWaves * kMaxBins; i += kSortThreads) (&counts[0][0])[i] = 0u;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
+    for (int r = 0; r < R; ++r) {
         const uint64_t alike = lanes_alike(digit[r], bits, live[r]);
         uint32_t before = 0u;
         if (live[r]) before = counts[wave][digit[r]];
@@ -132,13 +139,13 @@ __device__ __forceinline__ uint32_t key_of(const I *tokens, int64_t i, int64_t r
     return (uint32_t)(t >= 0 && t < rows ? t : rows);
 }
 
-// All passes for up to kBlockItems positions in one workgroup.
-template <typename I>
+// All passes for up to R * kSortThreads positions in one workgroup.
+template <typename I, int R>
 __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const I *__restrict__ tokens, int count, int64_t rows,
                                                                   int passes, int bits, uint32_t *__restrict__ keys,
                                                                   uint32_t *__restrict__ positions) {
-    __shared__ uint32_t key[kBlockItems];
-    __shared__ uint16_t order[kBlockItems];
+    __shared__ uint32_t key[R * kSortThreads];
+    __shared__ uint16_t order[R * kSortThreads];
     __shared__ uint32_t counts[kSortWaves][kMaxBins];
     __shared__ uint32_t totals[kMaxBins];
     __shared__ uint32_t scratch[kSortWaves];
@@ -149,12 +156,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const I *__res
     }
     __syncthreads();
     for (int p = 0; p < passes; ++p) {
-        uint32_t digit[kSortRounds], rank[kSortRounds];
-        uint16_t item[kSortRounds];
-        bool live[kSortRounds];
+        uint32_t digit[R], rank[R];
+        uint16_t item[R];
+        bool live[R];
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) {
-            const int i = wave * (64 * kSortRounds) + r * 64 + lane;
+        for (int r = 0; r < R; ++r) {
+            const int i = (wave * R + r) * 64 + lane;
             live[r] = i < count;
             item[r] = live[r] ? order[i] : (uint16_t)0;
             digit[r] = live[r] ? (key[item[r]] >> (p * bits)) & ((1u << bits) - 1u) : 0u;
@@ -162,7 +169,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const I *__res
         rank_items(digit, live, bits, counts, totals, rank);
         exclusive_scan(totals, 1 << bits, scratch);
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r)
+        for (int r = 0; r < R; ++r)
             if (live[r]) order[totals[digit[r]] + counts[wave][digit[r]] + rank[r]] = item[r];
         __syncthreads();
     }
@@ -179,10 +186,10 @@ struct SortArgs {
     const I *tokens;  // first pass, else NULL
     const uint32_t *keys_in, *positions_in;
     uint32_t *keys_out, *positions_out;
-    uint32_t *counts;  // [bin][blocks]
-    uint32_t *totals;  // [bin]
+    uint32_t *counts;  // [bin][blocks], made prefix sums over the blocks; `direct`: [block][bin], as counted
+    uint32_t *totals;  // [bin], not if `direct`
     int64_t count, rows;
-    int blocks, shift, bits;
+    int blocks, shift, bits, direct;
 };
 
 template <typename I>
@@ -197,12 +204,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs<I> a)
     for (int d = tid; d < bins; d += kSortThreads) bin[d] = 0u;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-        const int64_t i = (int64_t)blockIdx.x * kBlockItems + r * kSortThreads + tid;
+    for (int r = 0; r < kManyRounds; ++r) {
+        const int64_t i = (int64_t)blockIdx.x * kManyItems + r * kSortThreads + tid;
         if (i < a.count) atomicAdd(&bin[(sort_key(a, i) >> a.shift) & (uint32_t)(bins - 1)], 1u);  // whole numbers: any order
     }
     __syncthreads();
-    for (int d = tid; d < bins; d += kSortThreads) a.counts[(size_t)d * a.blocks + blockIdx.x] = bin[d];
+    for (int d = tid; d < bins; d += kSortThreads) a.counts[a.direct ? (size_t)blockIdx.x * bins + d : (size_t)d * a.blocks + blockIdx.x] = bin[d];
 }
 
 // A workgroup per digit: its counts over the blocks become exclusive prefix sums.
@@ -240,23 +247,37 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs<I> 
     __shared__ uint32_t base[kMaxBins];
     __shared__ uint32_t scratch[kSortWaves];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, bins = 1 << a.bits;
-    uint32_t key[kSortRounds], position[kSortRounds], digit[kSortRounds], rank[kSortRounds];
-    bool live[kSortRounds];
+    uint32_t key[kManyRounds], position[kManyRounds], digit[kManyRounds], rank[kManyRounds];
+    bool live[kManyRounds];
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-        const int64_t i = (int64_t)blockIdx.x * kBlockItems + wave * (64 * kSortRounds) + r * 64 + lane;
+    for (int r = 0; r < kManyRounds; ++r) {
+        const int64_t i = (int64_t)blockIdx.x * kManyItems + wave * (64 * kManyRounds) + r * 64 + lane;
         live[r] = i < a.count;
         key[r] = live[r] ? sort_key(a, i) : 0u;
         position[r] = live[r] ? (a.tokens ? (uint32_t)i : a.positions_in[i]) : 0u;
         digit[r] = (key[r] >> a.shift) & (uint32_t)(bins - 1);
     }
-    if (tid < bins) base[tid] = a.totals[tid];
+    uint32_t before = 0u;  // items of digit tid in earlier workgroups
+    if (tid < bins) {
+        if (a.direct) {
+            uint32_t all = 0u;
+            for (int b = 0; b < a.blocks; ++b) {
+                const uint32_t c = a.counts[(size_t)b * bins + tid];
+                if (b < (int)blockIdx.x) before += c;
+                all += c;
+            }
+            base[tid] = all;
+        } else {
+            before = a.counts[(size_t)tid * a.blocks + blockIdx.x];
+            base[tid] = a.totals[tid];
+        }
+    }
     __syncthreads();
     exclusive_scan(base, bins, scratch);
-    if (tid < bins) base[tid] += a.counts[(size_t)tid * a.blocks + blockIdx.x];
+    if (tid < bins) base[tid] += before;
     rank_items(digit, live, a.bits, counts, totals, rank);
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r)
+    for (int r = 0; r < kManyRounds; ++r)
         if (live[r]) {
             const uint32_t to = base[digit[r]] + counts[wave][digit[r]] + rank[r];
             a.keys_out[to] = key[r];
@@ -265,8 +286,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs<I> 
 }
 
 // ---- sums over runs of one token --------------------------------------------------------------------------------------
-constexpr int kAhead = 8;      // rows of dY in flight per lane
-constexpr int kZeroRows = 64;  // rows of dE per zero-filling workgroup
+constexpr int kAhead = 4;      // rows of dY in flight per lane (eight: 270 us instead of 245 for 65536 x 2048, fewer wavefronts fit)
+constexpr int kZeroRows = 32;  // rows of dE per zero-filling workgroup
 
 struct GradArgs {
     const uint32_t *keys, *positions;
@@ -286,14 +307,16 @@ __device__ __forceinline__ void finish_row(E *at, const float (&sum)[VEC], float
         load_f32<VEC>(at, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = v[e] + scale * sum[e];
+        store_f32<VEC>(at, v);
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = scale * sum[e];
+        store_f32<VEC, true>(at, v);
     }
-    store_f32<VEC>(at, v);
 }
 
-template <typename T, typename E, int VEC>
+// UNIFORM: a wavefront's lanes share their chunk (64 lanes and more a row), so that keys and positions are scalar loads.
+template <typename T, typename E, int VEC, bool UNIFORM>
 __global__ __launch_bounds__(256) void grad_chunks_kernel(GradArgs a, const T *__restrict__ dy, E *__restrict__ de) {
     if ((int64_t)blockIdx.x >= a.chunk_blocks) {  // zeros for the rows that no token names
         __shared__ uint8_t named[kZeroRows];
@@ -308,16 +331,22 @@ __global__ __launch_bounds__(256) void grad_chunks_kernel(GradArgs a, const T *_
             named[threadIdx.x] = row >= a.rows || (lo < a.count && (int64_t)a.keys[lo] == row);
         }
         __syncthreads();
-        const float zero[VEC] = {};
-        const int per = 256 / a.lanes, sub = threadIdx.x / a.lanes;
-        const int64_t col = ((int64_t)blockIdx.y * a.lanes + (threadIdx.x - sub * a.lanes)) * VEC;
-        if (col >= a.cols) return;
-        for (int r = sub; r < kZeroRows; r += per)
-            if (!named[r]) store_f32<VEC>(de + (row0 + r) * a.lde + col, zero);
+        // this workgroup's slab of columns, 16 bytes a lane (one element where rows are not made of whole vectors)
+        constexpr int kPiece = VEC == 1 ? 1 : 16 / (int)sizeof(E);
+        const float zero[kPiece] = {};
+        const int64_t slab = (int64_t)blockIdx.y * a.lanes * VEC;
+        const int64_t width = a.cols - slab < (int64_t)a.lanes * VEC ? a.cols - slab : (int64_t)a.lanes * VEC;
+        const int pieces = (int)(width / kPiece);
+        const int per = pieces >= 256 ? 1 : 256 / pieces, sub = threadIdx.x / pieces < per ? threadIdx.x / pieces : -1;
+        for (int r = pieces >= 256 ? 0 : sub; r >= 0 && r < kZeroRows; r += per)
+            if (!named[r])
+                for (int x = pieces >= 256 ? threadIdx.x : threadIdx.x - sub * pieces; x < pieces; x += 256)
+                    store_f32<kPiece, true>(de + (row0 + r) * a.lde + slab + (int64_t)x * kPiece, zero);
         return;
     }
     const int per = 256 / a.lanes, sub = threadIdx.x / a.lanes, lane = threadIdx.x - sub * a.lanes;
-    const int64_t chunk = (int64_t)blockIdx.x * per + sub;
+    int64_t chunk = (int64_t)blockIdx.x * per + sub;
+    if (UNIFORM) chunk = __builtin_amdgcn_readfirstlane((int)chunk);
     const int64_t col = ((int64_t)blockIdx.y * a.lanes + lane) * VEC;
     if (chunk >= a.chunks || col >= a.cols) return;
     const int64_t first = chunk * a.chunk;
@@ -423,8 +452,8 @@ int lanes_for(int64_t cols, int vec) {
 // Positions per chunk: short ones for few positions (a chunk's rows are read one batch after the other), longer ones for many
 // (fewer parts to store and join).
 int chunk_for(int64_t count) {
-    int c = kAhead;
-    while (c < 256 && (int64_t)c * 4096 < count) c *= 2;
+    int c = 8;
+    while (c < 256 && (int64_t)c * 1024 < count) c *= 2;
     return c;
 }
 
@@ -438,7 +467,7 @@ GradPlan plan_grad(int64_t count, int64_t rows) {
     while (total < 32 && (rows >> total) != 0) ++total;  // bits of the largest key, `rows`
     p.passes = (total + kMaxDigit - 1) / kMaxDigit;
     p.bits = (total + p.passes - 1) / p.passes;
-    p.blocks = (int)((count + kBlockItems - 1) / kBlockItems);
+    p.blocks = count <= kSmallItems ? 1 : (int)((count + kManyItems - 1) / kManyItems);
     p.chunk = chunk_for(count);
     p.chunks = (count + p.chunk - 1) / p.chunk;
     return p;
@@ -466,8 +495,13 @@ GradSpace lay_out(void *workspace, const GradPlan &p, int64_t count, int64_t col
 template <typename I>
 cn_status sort_tokens(const I *tokens, int64_t count, int64_t rows, const GradPlan &p, GradSpace &s, int *sorted, hipStream_t st) {
     if (p.blocks <= 1) {
-        hipLaunchKernelGGL((sort_small_kernel<I>), dim3(1), dim3(kSortThreads), 0, st, tokens, (int)count, rows, p.passes, p.bits,
-                           s.keys[0], s.positions[0]);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(1), dim3(kSortThreads), 0, st, tokens, (int)count, rows, p.passes, p.bits, s.keys[0], s.positions[0]);
+        };
+        if (count <= kSortThreads) go(sort_small_kernel<I, 1>);
+        else if (count <= 2 * kSortThreads) go(sort_small_kernel<I, 2>);
+        else if (count <= 4 * kSortThreads) go(sort_small_kernel<I, 4>);
+        else go(sort_small_kernel<I, kSmallRounds>);
         CN_HIP(hipGetLastError());
         *sorted = 0;
         return CN_OK;
@@ -475,9 +509,9 @@ cn_status sort_tokens(const I *tokens, int64_t count, int64_t rows, const GradPl
     for (int pass = 0; pass < p.passes; ++pass) {
         const int to = pass & 1, from = to ^ 1;
         SortArgs<I> a{pass == 0 ? tokens : nullptr, s.keys[from], s.positions[from], s.keys[to], s.positions[to],
-                      s.counts, s.totals, count, rows, p.blocks, pass * p.bits, p.bits};
+                      s.counts, s.totals, count, rows, p.blocks, pass * p.bits, p.bits, p.blocks <= kDirectBlocks};
         hipLaunchKernelGGL((sort_count_kernel<I>), dim3(p.blocks), dim3(kSortThreads), 0, st, a);
-        hipLaunchKernelGGL(sort_prefix_kernel, dim3(1 << p.bits), dim3(256), 0, st, s.counts, s.totals, p.blocks);
+        if (!a.direct) hipLaunchKernelGGL(sort_prefix_kernel, dim3(1 << p.bits), dim3(256), 0, st, s.counts, s.totals, p.blocks);
         hipLaunchKernelGGL((sort_scatter_kernel<I>), dim3(p.blocks), dim3(kSortThreads), 0, st, a);
         CN_HIP(hipGetLastError());
         *sorted = to;
@@ -498,8 +532,11 @@ cn_status run_grad(GradArgs a, const void *dy, void *de, hipStream_t st) {
         return CN_ERR_SHAPE;
     }
     if (a.chunk_blocks + zero_blocks == 0) return CN_OK;
-    hipLaunchKernelGGL((grad_chunks_kernel<T, E, VEC>), dim3((unsigned)(a.chunk_blocks + zero_blocks), (unsigned)slabs), dim3(256), 0,
-                       st, a, (const T *)dy, (E *)de);
+    const dim3 grid((unsigned)(a.chunk_blocks + zero_blocks), (unsigned)slabs);
+    if (a.lanes >= 64)
+        hipLaunchKernelGGL((grad_chunks_kernel<T, E, VEC, true>), grid, dim3(256), 0, st, a, (const T *)dy, (E *)de);
+    else
+        hipLaunchKernelGGL((grad_chunks_kernel<T, E, VEC, false>), grid, dim3(256), 0, st, a, (const T *)dy, (E *)de);
     if (a.chunks > 1)
         hipLaunchKernelGGL((grad_join_kernel<E, VEC>), dim3((unsigned)(a.chunks - 1), (unsigned)join_slabs), dim3(256), 0, st, a, (E *)de);
     CN_HIP(hipGetLastError());
