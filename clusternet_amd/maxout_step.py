@@ -14,6 +14,15 @@ Biases are inputs and are not updated.
 A sparse batch (the reference feeds its 2 % dense inputs as sparse matrices, source/Layer.cpp:250-255
 and 318-321) goes in as `sparse_input(X)`: the first layer's product and its weight gradient then run
 on the compressed rows of X and of X^T.
+
+A batch of words (the reference's windows of a language model, source/clusterKernels.cu:1497-1712) goes in as
+`token_input(table, tokens)`: the rows of a window's words side by side are the first layer's input, and the error that
+reaches them moves the table:
+
+    X = scale * E[tokens];  ... as above ...;  e0 = e1 W1^T;  E[v] -= table_rate * scale * sum of e0 over the words v
+
+`token_step` moves the two hidden weight matrices along their orthogonalised momentum and the last one by its 8-bit gradient.
+`quantize_params` and `answer` are for serving: the same forward pass from weights in 4 bits.
 """
 from . import _lib as L
 
@@ -30,8 +39,24 @@ def sparse_input(X):
     return SparseInput(csr, L.csr_transpose(csr))
 
 
+class TokenInput:
+    """Windows of words: the table (rows x D), the tokens (batch x window) and X (batch x window * D), their rows."""
+
+    def __init__(self, table, tokens, scale, X):
+        self.table, self.tokens, self.scale, self.X = table, tokens, scale, X
+
+
+def token_input(table, tokens, scale=1.0):
+    if tokens.dim() != 2:
+        raise ValueError("tokens must be batch x window")
+    X = L.embedding(table, tokens, scale)
+    return TokenInput(table, tokens, scale, X.view(X.shape[0], X.shape[1] * X.shape[2]))
+
+
 def forward(X, params, pool=2):
     W1, b1, W2, b2, W3, b3 = params
+    if isinstance(X, TokenInput):
+        X = X.X
     # bias and maxout are taken in one pass behind each product (inside it for the sparse first layer)
     if isinstance(X, SparseInput):
         h1, a1 = L.csr_gemm_bias_maxout(X.csr, W1, b1, pool)
@@ -46,8 +71,12 @@ def backward(X, onehot, params, p, cache, pool=2, absmax_out=None, defer_first=F
     """Weight gradients.  `absmax_out` = three one-element device tensors: the gradient products then
     also deliver max|gW|, which saves the abs-max pass in front of compression_8bit.
     `defer_first` (sparse input only): the first element of the result is the error signal e1 instead
-    of gW1 = X^T e1, for `coded_sparse_update`, which never stores that gradient."""
+    of gW1 = X^T e1, for `coded_sparse_update`, which never stores that gradient.
+    For a TokenInput the error signal at the words, e0 = e1 W1^T, is a fourth result."""
     W1, b1, W2, b2, W3, b3 = params
+    words = isinstance(X, TokenInput)
+    if words:
+        X = X.X
     h1, a1, h2, a2 = cache
     m1, m2, m3 = absmax_out if absmax_out is not None else (None, None, None)
     e3 = L.sub(p, onehot)
@@ -61,6 +90,8 @@ def backward(X, onehot, params, p, cache, pool=2, absmax_out=None, defer_first=F
         gW1 = L.csr_gemm(X.csr_t, e1, absmax_out=m1)
     else:
         gW1 = L.Tdot(X, e1, absmax_out=m1)
+    if words:
+        return gW1, gW2, gW3, L.dotT(e1, W1)
     return gW1, gW2, gW3
 
 
@@ -127,3 +158,38 @@ def step(X, onehot, params, rate, pool=2):
         else:
             coded_update(w, g, rate, prec=m)
     return p
+
+
+def table_update(X, e0, rate):
+    """E -= rate * dE in place, dE the gradient of the word table from the error signal e0 at the words of the TokenInput X;
+    rows of words that are not in the batch are not touched."""
+    return L.embedding_grad(e0.view(-1, X.table.shape[1]), X.tokens, X.table.shape[0], scale=-rate * X.scale, out=X.table,
+                            accumulate=True)
+
+
+def token_step(X, onehot, params, momenta, rate, table_rate, momentum_factor=0.95, coded_rate=0.01, pool=2):
+    """One step on a TokenInput: W1 and W2 along the orthogonalised `momenta` (two matrices of their shapes), W3 by its 8-bit
+    gradient, and the table."""
+    import torch
+    p, cache = forward(X, params, pool)
+    m3 = torch.empty(1, dtype=torch.float32, device=p.device)
+    gW1, gW2, gW3, e0 = backward(X, onehot, params, p, cache, pool, absmax_out=(None, None, m3))
+    for w, m, g in zip((params[0], params[2]), momenta, (gW1, gW2)):
+        L.muon_update(m, g, w, momentum_factor, rate)
+    coded_update(params[4], gW3, coded_rate, prec=m3)
+    table_update(X, e0, table_rate)
+    return p
+
+
+def quantize_params(params, group=128, zero_points=False):
+    """The parameters with their three matrices in 4 bits, for `answer`."""
+    return tuple(L.quantize_4bit(t, group, zero_points) if t.dim() == 2 else t for t in params)
+
+
+def answer(X, params4, pool=2):
+    """The probabilities of `forward` from the weights of `quantize_params`, which are never decoded to memory: X is a dense batch
+    (a row or a few dozen) or a TokenInput."""
+    W1, b1, W2, b2, W3, b3 = params4
+    h1, _ = L.bias_maxout(L.gemm_w4(X.X if isinstance(X, TokenInput) else X, W1), b1, pool)
+    h2, _ = L.bias_maxout(L.gemm_w4(h1, W2), b2, pool)
+    return L.softmax(L.add_row_vector(L.gemm_w4(h2, W3), b3))
