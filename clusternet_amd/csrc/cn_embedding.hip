@@ -8,7 +8,7 @@
 //   1. The positions are sorted by token, stably, by a radix sort of my own digits: ceil(log2(rows + 1)) bits in as many
 //      passes as digits of at most kMaxDigit bits need (two for a table of up to 2^18 rows).  A token outside the table
 //      takes the key `rows` and so comes last.  Up to kSmallItems positions one workgroup does all passes in LDS; beyond,
-//      a pass is two or three launches (count digits per block, for many blocks prefix sums per digit, scatter).
+//      a pass is three launches (count digits per block, prefix sums per digit over the blocks, scatter).
 //   2. The sorted list is cut into chunks of equal length, so a token that makes up a large share of the text costs no more
 //      than any other.  A group of lanes walks its chunk, adds the rows of dY in sorted order and writes each run of one
 //      token as it ends.  A run that crosses a chunk's border leaves its part in the workspace instead.
@@ -30,7 +30,6 @@ constexpr int kSmallItems = kSortThreads * kSmallRounds;      // 8192
 // a lane and 8 workgroups for 65536 tokens: 15 us a scatter).
 constexpr int kManyRounds = 2;
 constexpr int kManyItems = kSortThreads * kManyRounds;
-constexpr int kDirectBlocks = 64;  // up to so many, a workgroup adds up the counts of the others by itself: a launch less a pass
 constexpr int kMaxDigit = 9;                                  // bits of a digit
 constexpr int kMaxBins = 1 << kMaxDigit;
 
@@ -186,10 +185,10 @@ struct SortArgs {
     const I *tokens;  // first pass, else NULL
     const uint32_t *keys_in, *positions_in;
     uint32_t *keys_out, *positions_out;
-    uint32_t *counts;  // [bin][blocks], made prefix sums over the blocks; `direct`: [block][bin], as counted
-    uint32_t *totals;  // [bin], not if `direct`
+    uint32_t *counts;  // [bin][blocks]
+    uint32_t *totals;  // [bin]
     int64_t count, rows;
-    int blocks, shift, bits, direct;
+    int blocks, shift, bits;
 };
 
 template <typename I>
@@ -209,7 +208,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs<I> a)
         if (i < a.count) atomicAdd(&bin[(sort_key(a, i) >> a.shift) & (uint32_t)(bins - 1)], 1u);  // whole numbers: any order
     }
     __syncthreads();
-    for (int d = tid; d < bins; d += kSortThreads) a.counts[a.direct ? (size_t)blockIdx.x * bins + d : (size_t)d * a.blocks + blockIdx.x] = bin[d];
+    for (int d = tid; d < bins; d += kSortThreads) a.counts[(size_t)d * a.blocks + blockIdx.x] = bin[d];
 }
 
 // A workgroup per digit: its counts over the blocks become exclusive prefix sums.
@@ -257,24 +256,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs<I> 
         position[r] = live[r] ? (a.tokens ? (uint32_t)i : a.positions_in[i]) : 0u;
         digit[r] = (key[r] >> a.shift) & (uint32_t)(bins - 1);
     }
-    uint32_t before = 0u;  // items of digit tid in earlier workgroups
-    if (tid < bins) {
-        if (a.direct) {
-            uint32_t all = 0u;
-            for (int b = 0; b < a.blocks; ++b) {
-                const uint32_t c = a.counts[(size_t)b * bins + tid];
-                if (b < (int)blockIdx.x) before += c;
-                all += c;
-            }
-            base[tid] = all;
-        } else {
-            before = a.counts[(size_t)tid * a.blocks + blockIdx.x];
-            base[tid] = a.totals[tid];
-        }
-    }
+    if (tid < bins) base[tid] = a.totals[tid];
     __syncthreads();
     exclusive_scan(base, bins, scratch);
-    if (tid < bins) base[tid] += before;
+    if (tid < bins) base[tid] += a.counts[(size_t)tid * a.blocks + blockIdx.x];
     rank_items(digit, live, a.bits, counts, totals, rank);
 #pragma unroll
     for (int r = 0; r < kManyRounds; ++r)
@@ -509,9 +494,9 @@ cn_status sort_tokens(const I *tokens, int64_t count, int64_t rows, const GradPl
     for (int pass = 0; pass < p.passes; ++pass) {
         const int to = pass & 1, from = to ^ 1;
         SortArgs<I> a{pass == 0 ? tokens : nullptr, s.keys[from], s.positions[from], s.keys[to], s.positions[to],
-                      s.counts, s.totals, count, rows, p.blocks, pass * p.bits, p.bits, p.blocks <= kDirectBlocks};
+                      s.counts, s.totals, count, rows, p.blocks, pass * p.bits, p.bits};
         hipLaunchKernelGGL((sort_count_kernel<I>), dim3(p.blocks), dim3(kSortThreads), 0, st, a);
-        if (!a.direct) hipLaunchKernelGGL(sort_prefix_kernel, dim3(1 << p.bits), dim3(256), 0, st, s.counts, s.totals, p.blocks);
+        hipLaunchKernelGGL(sort_prefix_kernel, dim3(1 << p.bits), dim3(256), 0, st, s.counts, s.totals, p.blocks);
         hipLaunchKernelGGL((sort_scatter_kernel<I>), dim3(p.blocks), dim3(kSortThreads), 0, st, a);
         CN_HIP(hipGetLastError());
         *sorted = to;
