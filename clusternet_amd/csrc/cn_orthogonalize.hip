@@ -9,15 +9,27 @@
 //
 // The products are what this costs: 3 m^2 n + m^3 multiply-adds per step after the symmetry of A and A A (only tiles on and
 // above the diagonal are computed).  In fp32 the matrix cores give 157 TFLOP/s; here each operand is kept as two fp16
-// numbers, x 2^14 = hi + lo, and a product is the three fp16 products hi hi + hi lo + lo hi in fp32 accumulators.  What
-// is left out, lo lo, and the rounding of lo are 2^-22 of the product, so the result is as far from the exact one as plain
-// fp32 products leave it (emulated on the CPU for Gaussian, power-law and nearly rank-8 spectra: within 5 % of fp32's error).
-// The factor 2^14 keeps entries of all four matrices below 65504 (|X| <= 1.21, |A| <= 1.46, |P| <= 2.81) and lo above
-// the smallest fp16 number for entries down to 2^-13 of the largest.  a X stays outside the product, with X read back as
-// hi + lo: folding a into P's diagonal costs a factor of three in accuracy for nearly low-rank gradients.
-// For a bf16 result all steps but the last two take hi hi alone, a third of the work: the iteration contracts what
-// that costs (2^-12 per product), and 5 10^-5 to 8 10^-4 of |X| is left of it, under the 1.7 10^-3 of the result's own
-// rounding.  X itself keeps both parts in every step: with hi alone, gradients of low rank lose 4 10^-2.
+// numbers, x 2^14 = hi + lo (2^10 for P and Q), and a product is the three fp16 products hi hi + hi lo + lo hi in fp32
+// accumulators.  What is left out, lo lo, and the rounding of lo are 2^-22 of the product, so the result is about as far from
+// the exact one as plain fp32 products leave it (0.55 to 1.35 times as far at twelve sizes from 3000 x 16 to 16384 x 2048, up to
+// 1.8 times at tens of rows, where nothing averages out).  The factors keep entries below 65504 (|X| <= 1.21, |A|, |T| <= 1.46,
+// |P| <= 2.81, |Q| <= 41) and lo above the smallest fp16 number for entries down to 2^-13 of the largest.  a X stays outside
+// the product, with X read back as hi + lo: folding a into P's diagonal costs a factor of three in accuracy for nearly
+// low-rank gradients.
+//
+// For long matrices several steps are one: A, its polynomials and A' = p A p of the next step (p = a + P) commute, so a group of
+// steps runs on m x m matrices alone, Q = p'' p' p - a^3, and X <- a^3 X + Q X comes once at its end.  A group of g steps costs
+// 3 m^2 n + (4 g - 3) m^3 in place of g (3 m^2 n + m^3), at n = 4 m 42 % less for five steps as three and two.  A is computed from X
+// again after at most three steps in the beginning, where singular values grow, and two later on: with five steps in one group,
+// or three behind two, errors grow tenfold (emulated in 64 bits on Gaussian, orthogonal, rank-one, nearly low-rank spectra and
+// power laws), with three and two they stay at those of plain fp32.  Measured, steps alone -> in groups: 4096 x 16384 10.7 -> 6.8 ms,
+// 1000 x 4001 395 -> 342 us; equal by count at m = n, where it would only add launches.  Taken where the products' estimated
+// times add up to less (sizes_of).
+//
+// A gradient of 16 bits is its own hi if only the power of two of the scale is applied to it, so X0 X0^T is one product and Q X0
+// two, with nothing lost; the rest of the scale, in [1, 2), goes to their results (split_kernel).  (One product in place of
+// three in later steps too is not sound: hi alone is off by up to 2^-11 the same way in all equal entries, such as the
+// diagonal of A for orthogonal rows, and the next steps multiply that by ten: 5 10^-3 of |out| for 17 x 498.)
 //
 // Layout: a matrix is blocks of 256 rows, in them groups of 32 columns: a 128-byte line per row, 32 hi, then 32 lo.  A stage of
 // the product is then one line (or two) per row, all of them in a row in memory, and the tile in LDS is the fp32 kernel's
@@ -29,7 +41,7 @@
 // computes a whole tile applies the formula to its accumulators and writes the next operand in both orientations; parts of a
 // tile go to memory and a second kernel adds them in order.  Either way the result does not depend on scheduling.
 //
-// Measured (one MI355X): X^T P of 4096 x 16384 in 1.34 ms, 1.23 PFLOP/s of fp16 products with the write-out of X and X^T in it
+// Measured (one MI355X): X^T Q of 4096 x 16384 in 1.34 ms, 1.23 PFLOP/s of fp16 products with the write-out of X and X^T in it
 // (0.8 GB, of which little overlaps); the library's own 8192^3 fp16 product reaches 1.31 on the same card.  The chip runs
 // at its power limit (1.75 GHz on random numbers, 2.1 on zeros), so what would be won by fewer stalls is lost in clock.
 #include "cn_dtypes.h"
@@ -45,8 +57,7 @@ typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
-constexpr float kUnit = 16384.0f;                   // the stored number for 1
-constexpr float kProduct = 1.0f / (kUnit * kUnit);  // of an accumulator
+constexpr float kUnit = 16384.0f, kPolyUnit = 1024.0f;  // the stored number for 1: of X, A and T, and of P and Q
 constexpr int kPad = 256;                           // rows and columns are padded to whole tiles
 constexpr int kStage = 32;                          // of k
 
@@ -133,16 +144,29 @@ __global__ __launch_bounds__(256) void norm_kernel(Source s, double *parts) {
     if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 
-// X0 in both orientations, zeros in the padding.  A workgroup takes 64 x 64 elements of X (m x n).
+// X0 in both orientations, zeros in the padding.  A workgroup takes 64 x 64 elements of X (m x n).  `exact` (a gradient of 16
+// bits): only the power of two of the scale is applied, so that the stored numbers are the gradient's own, hi alone; the rest,
+// r in [1, 2), goes to the products of X0: factors = 1, r, r r.
 template <typename T>
-__global__ __launch_bounds__(256) void split_kernel(Source s, const double *parts, int part_count, int flip, int64_t mp, int64_t np,
-                                                    f16_t *x, f16_t *xt) {
+__global__ __launch_bounds__(256) void split_kernel(Source s, const double *parts, int part_count, int flip, int exact, int64_t mp,
+                                                    int64_t np, f16_t *x, f16_t *xt, float *factors) {
     __shared__ double scratch[4];
     __shared__ float tile[64][65];
     double sum = 0.0;
     for (int i = threadIdx.x; i < part_count; i += 256) sum += parts[i];
     sum = block_sum(sum, scratch);
-    const double to_unit = (double)kUnit / (sqrt(sum) + 1e-7);
+    double to_unit = (double)kUnit / (sqrt(sum) + 1e-7);
+    float rest = 1.0f;
+    if (exact && to_unit > 0.0) {  // neither 0 nor NaN: the gradient is finite
+        int exponent;
+        rest = 2.0f * (float)frexp(to_unit, &exponent);
+        to_unit = ldexp(1.0, exponent - 1);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        factors[0] = 1.0f;
+        factors[1] = rest;
+        factors[2] = rest * rest;
+    }
     const int64_t blocks_n = np / 64;
     const int64_t i0 = blockIdx.x / blocks_n * 64, j0 = blockIdx.x % blocks_n * 64;  // of X
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -173,10 +197,11 @@ __global__ __launch_bounds__(256) void split_kernel(Source s, const double *part
 // ---- products ------------------------------------------------------------------------------------------------------------
 // D[i][j] = sum over k of U[i][k] V[j][k], both operands split, and what becomes of it.
 enum Finish {
-    GRAM = 0,  // A, symmetric
-    POLY = 1,  // P = b A + c A A, symmetric; D = A A
-    STEP = 2,  // X <- a X + P X, both orientations; D = X^T P, n x m
-    LAST = 3   // the same, into the result
+    GRAM = 0,  // y D, symmetric
+    POLY = 1,  // x old + y D, symmetric
+    SUM = 2,   // x old + x2 old2 + y D, symmetric
+    STEP = 3,  // X <- x X + y D^T, both orientations; D = X^T P, n x m
+    LAST = 4   // the same, into the result
 };
 //
 // Units of work: a group of `count` consecutive tiles, each cut along k into `parts`; workgroup w of a group takes part
@@ -194,8 +219,10 @@ struct Product {
     int triangle;            // the result is symmetric: only tiles with j >= i
     Group group[kMaxGroups];  // unused ones: all 0
     float *parts;            // TILE x TILE numbers per unit of a group with more than one part per tile
-    const f16_t *old;        // POLY: A;  STEP, LAST: X
-    f16_t *to;               // GRAM, POLY: A, P;  STEP: X (its own elements only, so in place)
+    const f16_t *old, *old2;  // STEP, LAST: X
+    float x, x2, y;           // in stored units
+    const float *factor;      // x and y are multiplied by this
+    f16_t *to;                // symmetric results; STEP: X (its own elements only, so in place)
     f16_t *to_t;             // STEP: X^T of the next step (this one's is an operand)
     int64_t to_cols, to_t_cols;
     void *out;               // LAST: the result, as the caller has it, or the weights
@@ -221,7 +248,7 @@ constexpr int lines_of(int tile, int terms) {
     return terms == 1 ? 1 : tile == 256 ? Shape<256>::LINES : tile == 128 ? Shape<128>::LINES : Shape<64>::LINES;
 }
 // k of a stage.
-constexpr int depth_of(int tile, int terms) { return lines_of(tile, terms) * (terms == 3 ? 32 : 64); }
+constexpr int depth_of(int tile, int terms) { return lines_of(tile, terms) * (terms == 1 ? 64 : 32); }
 
 __device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ ((row >> 3) & 3); }
 
@@ -293,17 +320,17 @@ struct Cursor {
     }
 };
 
-// What a lane needs of the old X or A for a 32 x 32 block: rows j, along i.
+// What a lane needs of an old matrix for a 32 x 32 block: rows j, along i.
 struct Old {
     f16x4 hi[4], lo[4];
 };
 template <int FINISH>
-__device__ __forceinline__ void load_old(const Product &g, int64_t i0, int64_t j0, Old &o) {
+__device__ __forceinline__ void load_old(const Product &g, const f16_t *from, int64_t i0, int64_t j0, Old &o) {
     if (FINISH == GRAM) return;
     const int sub = (threadIdx.x & 63) >> 3, quad = threadIdx.x & 7;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        const f16_t *at = g.old + split_at(j0 + 8 * p + sub, i0 + 4 * quad, g.to_cols);
+        const f16_t *at = from + split_at(j0 + 8 * p + sub, i0 + 4 * quad, g.to_cols);
         o.hi[p] = *reinterpret_cast<const f16x4 *>(at);
         o.lo[p] = *reinterpret_cast<const f16x4 *>(at + 32);
     }
@@ -346,12 +373,14 @@ __device__ __forceinline__ void write_result(const Product &g, int64_t row, int6
 }
 
 // One 32 x 32 block of D, corner (i0, j0), from a wavefront's sums as the matrix instructions leave them: number r of lane
-// (half, l) is row 8 (r / 4) + 4 half + r % 4, column l.  X, A and P are read and written as rows j, along i (A, A A and P are
-// symmetric, D = X^T P belongs to row j of X), then, with `mirror`, as rows i, along j.  `stage`: 4 KiB of LDS of the
+// (half, l) is row 8 (r / 4) + 4 half + r % 4, column l.  Matrices are read and written as rows j, along i (symmetric ones may be,
+// D = X^T P belongs to row j of X), then, with `mirror`, as rows i, along j.  `stage`: 4 KiB of LDS of the
 // wavefront's own, [j][i] in 16-byte columns xor-swizzled by j / 2, so that eight lanes write 64 bytes of a row at a time.
 template <int FINISH>
-__device__ __forceinline__ void finish_block(const Product &g, const f32x16 &sum, const Old &old, int64_t i0, int64_t j0, bool mirror,
-                                             float *stage) {
+__device__ __forceinline__ void finish_block(const Product &g, float factor, const f32x16 &sum, const Old &old, int64_t i0, int64_t j0,
+                                             bool mirror, float *stage) {
+    Old old2;
+    if (FINISH == SUM) load_old<FINISH>(g, g.old2, i0, j0, old2);
     const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -361,7 +390,7 @@ __device__ __forceinline__ void finish_block(const Product &g, const f32x16 &sum
     __builtin_amdgcn_wave_barrier();
     const int sub = lane >> 3, quad = lane & 7;
     constexpr bool last = FINISH == LAST;
-    const float x = FINISH == POLY ? kB : kA, y = (FINISH == POLY ? kC : 1.0f) * (kProduct * kUnit);
+    const float x = g.x * factor, y = g.y * factor;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const int j = 8 * p + sub;
@@ -371,6 +400,7 @@ __device__ __forceinline__ void finish_block(const Product &g, const f32x16 &sum
         for (int e = 0; e < 4; ++e) {
             v[e] *= y;
             if (FINISH != GRAM) v[e] = x * ((float)old.hi[p][e] + (float)old.lo[p][e]) + v[e];
+            if (FINISH == SUM) v[e] = g.x2 * ((float)old2.hi[p][e] + (float)old2.lo[p][e]) + v[e];
         }
         const float w[4] = {v[0], v[1], v[2], v[3]};
         if (!last) {
@@ -430,6 +460,7 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
     const unsigned W = gridDim.x, xcd = blockIdx.x % 8u, idx = blockIdx.x / 8u, per = W / 8u, rem = W % 8u;
     const int w = (int)(xcd * per + (xcd < rem ? xcd : rem) + idx);
     const Units units(g, w);
+    const float factor = __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(*g.factor)));
     Cursor at, ahead;  // the stage that is computed, the one that is requested next
     bool more = ahead.next_unit(g, units);  // something is left to request
     int requested = 0;                      // stages requested and not yet computed
@@ -439,7 +470,7 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
     for (int j = 0; j < kLoads; ++j) {
         const int at = (j * kWaves + wave) * 8 + (lane >> 3), row = at % TILE;
         const uint32_t column = (uint32_t)((lane & 7) ^ swizzle(row));
-        off[j] = (uint32_t)(at / TILE) * (256 * 128) + (uint32_t)row * 128 + (TERMS == 3 ? column * 16 : (column >> 2) * (256 * 128) + (column & 3) * 16);
+        off[j] = (uint32_t)(at / TILE) * (256 * 128) + (uint32_t)row * 128 + (TERMS > 1 ? column * 16 : (column >> 2) * (256 * 128) + (column & 3) * 16);
     }
     // Inline assembly because the compiler would make every later LDS read wait for a load it knows to write LDS; the wait
     // is at the head of each stage.  No output registers.
@@ -480,7 +511,7 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
     f32x16 acc[S::FM][S::FN];
 
     // Lane (half, i) reads k = 16 s + 8 half .. + 7 of row i: 16-byte column 2 s + half of its row, lo four columns further.
-    constexpr int kSteps = TERMS == 3 ? 2 : 4;
+    constexpr int kSteps = TERMS > 1 ? 2 : 4;
     auto frag = [&](int base, int row, int quad) {
         return *reinterpret_cast<const f16x8 *>(smem + base + row * 128 + ((quad ^ swizzle(row)) << 4));
     };
@@ -499,7 +530,7 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
             for (int ni = 0; ni < S::FN; ++ni) {
                 const int row = (wave_j * S::FN + ni) * 32 + l32;
                 vh[s & 1][ni] = frag(bv, row, 2 * s + half);
-                if (TERMS == 3) vl[s & 1][ni] = frag(bv, row, 4 + 2 * s + half);
+                if (TERMS > 1) vl[s & 1][ni] = frag(bv, row, 4 + 2 * s + half);
             }
         }
         const int row = (wave_i * S::FM + mi) * 32 + l32;
@@ -528,7 +559,7 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
             for (int ni = 0; ni < S::FN; ++ni) {
                 const int row = (wave_j * S::FN + ni) * 32 + l32;
                 bh[ni] = frag(bv, row, column);
-                if (TERMS == 3) bl[ni] = frag(bv, row, 4 + column);
+                if (TERMS > 1) bl[ni] = frag(bv, row, 4 + column);
             }
 #pragma unroll
             for (int mi = 0; mi < S::FM; ++mi) {
@@ -640,7 +671,7 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
         // registers are picked by a branch.  Old values are requested a block ahead, in front of the stores of the block before:
         // the counter that a load is waited for with would otherwise drain them first.
         Old old, next;
-        if (at.slot < 0 && from < until) load_old<FINISH>(g, place_i(from), place_j(from), old);
+        if (at.slot < 0 && from < until) load_old<FINISH>(g, g.old, place_i(from), place_j(from), old);
 #pragma unroll 1
         for (int b = from; b < until; ++b) {
             f32x16 sum;
@@ -652,8 +683,8 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
                 }
             });
             if (at.slot < 0) {
-                if (b + 1 < until) load_old<FINISH>(g, place_i(b + 1), place_j(b + 1), next);
-                finish_block<FINISH>(g, sum, old, place_i(b), place_j(b), mirror, own);
+                if (b + 1 < until) load_old<FINISH>(g, g.old, place_i(b + 1), place_j(b + 1), next);
+                finish_block<FINISH>(g, factor, sum, old, place_i(b), place_j(b), mirror, own);
                 old = next;
             } else {
                 float *out = g.parts + (size_t)at.slot * TILE * TILE;
@@ -683,7 +714,7 @@ __global__ __launch_bounds__(256) void join_kernel(Product g, int from) {
     tile_place(tile, g.tiles_j, g.triangle, ti, tj);
     const int64_t i0 = (int64_t)ti * TILE + block / kSide * 32, j0 = (int64_t)tj * TILE + block % kSide * 32;
     Old old;
-    load_old<FINISH>(g, i0, j0, old);
+    load_old<FINISH>(g, g.old, i0, j0, old);
     f32x16 sum;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
@@ -696,7 +727,7 @@ __global__ __launch_bounds__(256) void join_kernel(Product g, int from) {
             for (int e = 0; e < 4; ++e) sum[4 * q + e] += x[e];
         }
     }
-    finish_block<FINISH>(g, sum, old, i0, j0, !(g.triangle && ti == tj), stage[wave]);
+    finish_block<FINISH>(g, *g.factor, sum, old, i0, j0, !(g.triangle && ti == tj), stage[wave]);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -748,14 +779,14 @@ Cut cut_with(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, int t
 // epilogue, storing a part; a launch takes 4 us more than what runs in it, the parts are written and read at about 8 TB/s together.
 double cost_of(const Cut &c, int terms) {
     const int size = c.tile == 256 ? 0 : c.tile == 128 ? 1 : 2;
-    static const double stage[3][2] = {{2.1, 2.42}, {1.2, 1.55}, {0.55, 0.53}};  // [size][parts of the operands]
+    static const double stage[3][3] = {{2.1, 1.75, 2.42}, {1.2, 1.2, 1.55}, {0.55, 0.5, 0.53}};  // [size][products - 1]
     static const double finish[3] = {13.0, 3.0, 1.5}, store[3] = {3.0, 2.0, 1.0};
     double t = 4.0;
     int busy = 0;
     for (const Group &g : c.group) {
         if (g.count == 0) continue;
         // a chip that is not full runs at a higher clock
-        const double one = stage[size][terms == 3] * (size < 2 && g.count * g.parts < 200 ? 0.72 : 1.0);
+        const double one = stage[size][terms - 1] * (size < 2 && g.count * g.parts < 200 ? 0.72 : 1.0);
         t += g.rounds * (c.stages / (double)g.parts * one + (g.parts > 1 ? store[size] : finish[size]));
         busy += g.parts > 1 ? g.count * g.parts : 0;
     }
@@ -778,16 +809,15 @@ Cut cut_product(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, in
 }
 
 struct Space {
-    f16_t *x, *xt[2], *a, *p;
-    float *parts;
+    f16_t *x, *xt[2], *a, *b[3];
+    float *parts, *factors;
     double *norms;
     size_t bytes;
 };
-constexpr int kGram = 0, kSquare = 1, kApply = 2;  // the products of a step
 struct Sizes {
     int64_t m, n, mp, np;
-    int flip;
-    Cut cut[2][3];  // [products of one part, of three][product]
+    int flip, grouped;
+    Cut gram[2], square, apply[2];  // [all parts of X, or of an exact X0 hi alone]
 };
 Sizes sizes_of(int64_t rows, int64_t cols) {
     Sizes z;
@@ -796,31 +826,33 @@ Sizes sizes_of(int64_t rows, int64_t cols) {
     z.n = z.flip ? rows : cols;
     z.mp = padded(z.m);
     z.np = padded(z.n);
-    for (int t = 0; t < 2; ++t) {
-        const int terms = t == 0 ? 1 : 3;
-        z.cut[t][kGram] = cut_product(z.m, z.m, z.n, true, terms);
-        z.cut[t][kSquare] = cut_product(z.m, z.m, z.m, true, terms);
-        z.cut[t][kApply] = cut_product(z.n, z.m, z.m, false, terms);
+    z.square = cut_product(z.m, z.m, z.m, true, 3);
+    for (int exact = 0; exact < 2; ++exact) {
+        z.gram[exact] = cut_product(z.m, z.m, z.n, true, exact ? 1 : 3);
+        z.apply[exact] = cut_product(z.n, z.m, z.m, false, exact ? 2 : 3);
     }
+    // Steps in groups, by the products of five steps: 2 of each size n and 14 small ones against 5 and 5.
+    const double large = cost_of(z.gram[0], 3) + cost_of(z.apply[0], 3), small = cost_of(z.square, 3);
+    z.grouped = 2 * large + 14 * small < 5 * (large + small);
     return z;
 }
 
 Space lay_out(void *workspace, const Sizes &z) {
     Carver c(workspace);
-    Space s;
+    Space s{};
     s.x = c.take<f16_t>((size_t)z.mp * z.np * 2);
     s.xt[0] = c.take<f16_t>((size_t)z.mp * z.np * 2);
     s.xt[1] = c.take<f16_t>((size_t)z.mp * z.np * 2);
     s.a = c.take<f16_t>((size_t)z.mp * z.mp * 2);
-    s.p = c.take<f16_t>((size_t)z.mp * z.mp * 2);
+    for (int i = 0; i < (z.grouped ? 3 : 1); ++i) s.b[i] = c.take<f16_t>((size_t)z.mp * z.mp * 2);
     size_t parts = 0;
-    for (const auto &of_terms : z.cut)
-        for (const Cut &cut : of_terms) {
-            const size_t need = (size_t)cut.slots * cut.tile * cut.tile;
-            if (need > parts) parts = need;
-        }
+    for (const Cut *cut : {&z.gram[0], &z.gram[1], &z.square, &z.apply[0], &z.apply[1]}) {
+        const size_t need = (size_t)cut->slots * cut->tile * cut->tile;
+        if (need > parts) parts = need;
+    }
     s.parts = c.take<float>(parts);
     s.norms = c.take<double>(kNormBlocks);
+    s.factors = c.take<float>(3);
     s.bytes = c.used;
     return s;
 }
@@ -837,15 +869,10 @@ cn_status run_product(const Product &g, const Cut &c, int device, hipStream_t st
     CN_HIP(hipGetLastError());
     return CN_OK;
 }
-template <int FINISH>
-cn_status run_product(const Product &g, const Cut &c, int terms, int device, hipStream_t st) {
-    if (terms == 3 || FINISH == LAST)  // the last steps are always products of all parts
-        return c.tile == 256 ? run_product<256, 3, FINISH>(g, c, device, st) : c.tile == 128 ? run_product<128, 3, FINISH>(g, c, device, st)
-                                                                                             : run_product<64, 3, FINISH>(g, c, device, st);
-    if constexpr (FINISH != LAST)
-        return c.tile == 256 ? run_product<256, 1, FINISH>(g, c, device, st) : c.tile == 128 ? run_product<128, 1, FINISH>(g, c, device, st)
-                                                                                             : run_product<64, 1, FINISH>(g, c, device, st);
-    return CN_ERR_ARG;
+template <int TERMS, int FINISH>
+cn_status run_product(const Product &g, const Cut &c, int device, hipStream_t st) {
+    return c.tile == 256 ? run_product<256, TERMS, FINISH>(g, c, device, st) : c.tile == 128 ? run_product<128, TERMS, FINISH>(g, c, device, st)
+                                                                                             : run_product<64, TERMS, FINISH>(g, c, device, st);
 }
 
 struct Result {
@@ -856,44 +883,91 @@ struct Result {
     float keep, rate;
 };
 
+constexpr int kFirstGroup = 3, kGroup = 2;  // steps
+
 template <typename T>
 cn_status newton_schulz(const Source &src, int steps, const Result &res, const Sizes &z, const Space &s, int device, hipStream_t st) {
     const int64_t norm_tiles = ((src.cols + 255) / 256) * ((src.rows + 15) / 16);
     const int norm_blocks = (int)(norm_tiles < kNormBlocks ? norm_tiles : kNormBlocks);
+    const int exact = sizeof(T) == 2 && !src.momentum;
     hipLaunchKernelGGL((norm_kernel<T>), dim3(norm_blocks), dim3(256), 0, st, src, s.norms);
     hipLaunchKernelGGL((split_kernel<T>), dim3((unsigned)((z.mp / 64) * (z.np / 64))), dim3(256), 0, st, src, s.norms, norm_blocks, z.flip,
-                       z.mp, z.np, s.x, s.xt[0]);
+                       exact, z.mp, z.np, s.x, s.xt[0], s.factors);
     CN_HIP(hipGetLastError());
-    int at = 0;  // which X^T is current
-    for (int step = 0; step < steps; ++step) {
-        for (int which = GRAM; which <= STEP; ++which) {
-            const bool full = res.dtype != CN_BF16 || step + 2 >= steps;
-            const Cut &c = z.cut[full][which];
-            Product g{};
-            g.u = which == GRAM ? s.x : which == POLY ? s.a : s.xt[at];
-            g.v = which == GRAM ? s.x : which == POLY ? s.a : s.p;
-            g.u_cols = which == GRAM ? z.np : z.mp;
-            g.v_cols = g.u_cols;
-            g.tiles_j = c.tiles_j;
-            g.stages = c.stages;
-            g.triangle = which != STEP;
-            for (int i = 0; i < kMaxGroups; ++i) g.group[i] = c.group[i];
-            g.parts = s.parts;
-            g.old = which == POLY ? s.a : s.x;
-            g.to = which == GRAM ? s.a : which == POLY ? s.p : s.x;
-            g.to_cols = which == STEP ? z.np : z.mp;
-            g.to_t = s.xt[at ^ 1];
-            g.to_t_cols = z.mp;
-            g.out = res.out; g.out_dtype = res.dtype; g.ldo = res.ldo; g.m = z.m; g.n = z.n; g.flip = z.flip;
-            g.wide = res.ldo % 4 == 0 && aligned_to(res.out, 4 * dtype_bytes(res.dtype));
-            g.update = res.update; g.keep = res.keep; g.rate = res.rate;
-            const int terms = full ? 3 : 1;
-            const cn_status status = which == GRAM ? run_product<GRAM>(g, c, terms, device, st)
-                                   : which == POLY ? run_product<POLY>(g, c, terms, device, st)
-                                   : step + 1 < steps ? run_product<STEP>(g, c, terms, device, st) : run_product<LAST>(g, c, 3, device, st);
-            if (status != CN_OK) return status;
+    Product base{};
+    base.parts = s.parts;
+    base.to_t_cols = z.mp;
+    base.factor = s.factors;
+    base.out = res.out; base.out_dtype = res.dtype; base.ldo = res.ldo; base.m = z.m; base.n = z.n; base.flip = z.flip;
+    base.wide = res.ldo % 4 == 0 && aligned_to(res.out, 4 * dtype_bytes(res.dtype));
+    base.update = res.update; base.keep = res.keep; base.rate = res.rate;
+    auto with = [&](const Cut &c, const f16_t *u, const f16_t *v, int64_t depth) {
+        Product g = base;
+        g.u = u; g.v = v;
+        g.u_cols = g.v_cols = depth;
+        g.tiles_j = c.tiles_j;
+        g.stages = c.stages;
+        for (int i = 0; i < kMaxGroups; ++i) g.group[i] = c.group[i];
+        return g;
+    };
+    // to = x old + y U V of symmetric matrices that commute, in stored units; with old2 SUM.
+    auto square = [&](const f16_t *u, const f16_t *v, const f16_t *old, float x, const f16_t *old2, float x2, float y, f16_t *to) {
+        Product g = with(z.square, u, v, z.mp);
+        g.triangle = 1;
+        g.old = old; g.old2 = old2;
+        g.x = x; g.x2 = x2; g.y = y;
+        g.to = to;
+        g.to_cols = z.mp;
+        return old2 ? run_product<3, SUM>(g, z.square, device, st) : run_product<3, POLY>(g, z.square, device, st);
+    };
+    constexpr float kMixed = kUnit / (kUnit * kPolyUnit);  // y of a product of an operand in each unit whose result is in kUnit
+    int at = 0;                                            // which X^T is current
+    for (int done = 0; done < steps;) {
+        const int most = !z.grouped ? 1 : done == 0 ? kFirstGroup : kGroup, count = steps - done < most ? steps - done : most;
+        const bool hi_alone = exact && done == 0;
+        Product g = with(z.gram[hi_alone], s.x, s.x, z.np);
+        g.triangle = 1;
+        g.y = 1.0f / kUnit;
+        g.factor = s.factors + (done == 0 ? 2 : 0);
+        g.to = s.a;
+        g.to_cols = z.mp;
+        cn_status status = hi_alone ? run_product<1, GRAM>(g, z.gram[1], device, st) : run_product<3, GRAM>(g, z.gram[0], device, st);
+        auto poly = [&](f16_t *to) {
+            return square(s.a, s.a, s.a, kB * kPolyUnit / kUnit, nullptr, 0.0f, kC * kPolyUnit / (kUnit * kUnit), to);
+        };
+        // p: the step's polynomial, q: the group's, t: p A
+        f16_t *p = s.b[0], *q = s.b[0];
+        float q0 = kA;
+        if (status == CN_OK) status = poly(p);
+        for (int k = 1; k < count && status == CN_OK; ++k) {
+            f16_t *t = s.b[0], *next = s.b[0];
+            for (f16_t *b : s.b)
+                if (b != p && b != q) t = b;
+            status = square(s.a, p, s.a, kA, nullptr, 0.0f, kMixed, t);
+            if (status == CN_OK) status = square(p, t, t, kA, nullptr, 0.0f, kMixed, s.a);
+            p = t;
+            if (status == CN_OK) status = poly(p);
+            for (f16_t *b : s.b)
+                if (b != p && b != q) next = b;
+            if (status == CN_OK) status = square(p, q, p, q0, q, kA, 1.0f / kPolyUnit, next);
+            q = next;
+            q0 *= kA;
         }
+        if (status != CN_OK) return status;
+        const bool last = done + count == steps, two = hi_alone && !last;
+        const Cut &c = z.apply[two];
+        g = with(c, s.xt[at], q, z.mp);
+        g.old = s.x;
+        g.x = q0;
+        g.y = kMixed;
+        g.factor = s.factors + (done == 0 ? 1 : 0);
+        g.to = s.x;
+        g.to_cols = z.np;
+        g.to_t = s.xt[at ^ 1];
+        status = last ? run_product<3, LAST>(g, c, device, st) : two ? run_product<2, STEP>(g, c, device, st) : run_product<3, STEP>(g, c, device, st);
+        if (status != CN_OK) return status;
         at ^= 1;
+        done += count;
     }
     return CN_OK;
 }

@@ -4,10 +4,9 @@ Tolerance.  A step maps singular values by p(s) = a s + b s^3 + c s^5; as a map 
 Frobenius norm is max |p'| on [0, 1.21], which is below 4.2.  An error of relative size e in each step is therefore at most
 e (4.2^5 - 1) / 3.2 = 408 e after five.  A step's own errors are roundings of 2^-24 (fp32 sums) and 2^-22 (the two-part operands) at a
 handful of places (A, A A, P, the product, the stored X), independent from element to element: e = 2^-21 covers eight of
-them.  So 408 * 2^-21 = 2e-4 of |out|_F, and for 16-bit results half a step of each element on top (for bfloat16, 2^-8, that is
-more than the 1e-3 its shorter products may cost: their roundings of 2^-12 in the first three steps pass through p of the
-last two, whose slope on the interval that they are in by then, 0.7 to 1.2, is what contracts them).  (One lost
-part of an operand is 2^-12 per product, and shows as 1e-3 to 3e-3.)"""
+them.  So 408 * 2^-21 = 2e-4 of |out|_F, and for 16-bit results half a step of each element on top.  Long matrices take steps in
+groups, which carry A along in place of X: A' = p A p passes an error of A on with at most a^2 = 11.9, X X^T of a step's X with
+4.2^2.  (One lost part of an operand is 2^-12 per product, and shows as 1e-3 to 3e-3.)"""
 import numpy as np
 import pytest
 
@@ -46,6 +45,13 @@ def _gradient(torch, rows, cols, seed, kind="noise"):
     if kind == "strong":  # a few directions far above the rest
         k = min(4, rows, cols)
         g = 0.02 * g + torch.randn(rows, k, generator=gen, device="cuda") @ torch.randn(k, cols, generator=gen, device="cuda")
+    if kind == "identity":  # all entries that count alike, as all singular values
+        g = torch.eye(rows, cols, device="cuda")
+    if kind == "constant":
+        g = torch.full_like(g, 0.37)
+    if kind == "orthogonal":
+        g = torch.linalg.qr((g if rows >= cols else g.T).contiguous()).Q
+        g = (g if rows >= cols else g.T).contiguous()
     if kind == "repeated" and rows > 1:  # rank deficient
         g[rows - rows // 2:] = g[:rows // 2].clone()
     return g
@@ -84,11 +90,33 @@ def test_16_bit_gradients(torch, dtype, rows, cols):
     _close(torch, cn.orthogonalize(G, out=torch.empty(rows, cols, device="cuda")), want)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows,cols", [(17, 498), (300, 300), (100, 1700), (700, 2900), (4500, 1030)])
+@pytest.mark.parametrize("kind", ["identity", "constant", "orthogonal"])
+def test_equal_entries_and_singular_values(torch, rows, cols, dtype, kind):
+    """Where roundings do not average out: the same in every entry, or passed on with the same slope.  In 32 bits of result too, so
+    that nothing hides behind its rounding."""
+    import clusternet_amd as cn
+    G = _gradient(torch, rows, cols, 11, kind).to(getattr(torch, dtype))
+    want = _exact(torch, G)
+    _close(torch, cn.orthogonalize(G), want)
+    _close(torch, cn.orthogonalize(G, out=torch.empty(rows, cols, device="cuda")), want)
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 8])
 def test_numbers_of_steps(torch, steps):
     import clusternet_amd as cn
     G = _gradient(torch, 200, 150, 8)
     _close(torch, cn.orthogonalize(G, steps=steps), _exact(torch, G, steps), steps)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7])
+@pytest.mark.parametrize("rows,cols", [(700, 2900), (4500, 600)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_numbers_of_steps_of_long_matrices(torch, rows, cols, dtype, steps):
+    import clusternet_amd as cn
+    G = _gradient(torch, rows, cols, 9).to(getattr(torch, dtype))
+    _close(torch, cn.orthogonalize(G, steps=steps, out=torch.empty(rows, cols, device="cuda")), _exact(torch, G, steps), steps)
 
 
 def test_against_plain_32_bits(torch):
