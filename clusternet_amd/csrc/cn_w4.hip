@@ -138,11 +138,13 @@ __device__ __forceinline__ void load_eight(const T *row, int64_t k, int64_t K, b
 }
 
 // NT tiles of 16 columns and MB blocks of 16 rows per workgroup, WAVES wavefronts that split K, GROUPS scales per 128 rows.
-// Codes and scales are requested kAhead tiles of 128 rows before they are used, A of a single block of rows one tile.
+// Codes and scales are requested kAhead tiles of 128 rows before they are used, A of a single block of rows one tile, of two
+// blocks half a tile at a time (64 k: whole lines of a row of 16 bits at once, before the other wavefronts' rows push
+// them out of the cache).
 template <typename T, int NT, int MB, int WAVES, int GROUPS>
 __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
     using Q = Kind<T>;
-    constexpr int kRaw = sizeof(T) / 2, kParts = Q::kParts, kAhead = MB > 1 ? 1 : 2, kSpan = 4 / GROUPS;
+    constexpr int kRaw = sizeof(T) / 2, kParts = Q::kParts, kAhead = 2, kSpan = 4 / GROUPS;
     constexpr bool kAheadA = MB == 1;
     extern __shared__ __attribute__((aligned(16))) float sums[];  // [WAVES][MB][NT][64][4]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
         float scale[NT][GROUPS], zero[NT][GROUPS];
     };
     Slot slots[kAhead];
-    u32x4 ahead_a[2][kAheadA ? 4 : 1][kRaw];
+    u32x4 ahead_a[2][kAheadA ? 4 : 1][kRaw], half_a[2][MB][kRaw];
     const int64_t full = g.vec_a ? g.K / kTileK : 0;  // tiles of A that are read 16 bytes at a time; the others element by element
     const int kw = __builtin_amdgcn_readfirstlane((int)(full < k0 ? k0 : full < k1 ? full : k1));
     auto request = [&](Slot &s, int kb) {
@@ -196,6 +198,14 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
             for (int q = 0; q < 4; ++q) load_eight<true>(row[0], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, true, a[q]);
         }
     };
+    auto request_half = [&](int64_t k) {
+        if constexpr (!kAheadA) {
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) load_eight<true>(row[b], k + 32 * e, g.K - 8 * h, true, half_a[e][b]);
+        }
+    };
 
     f32x4 total[MB][NT];
 #pragma unroll
@@ -204,7 +214,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
         for (int t = 0; t < NT; ++t) total[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     const u32x4 ones = {Q::kOnes, Q::kOnes, Q::kOnes, Q::kOnes};
 
-    auto consume = [&](const Slot &s, const u32x4 (&a)[kAheadA ? 4 : 1][kRaw], int kb, auto whole) {
+    auto consume = [&](const Slot &s, const u32x4 (&a)[kAheadA ? 4 : 1][kRaw], int kb, int next, auto whole) {
         constexpr bool kWhole = decltype(whole)::value != 0;
         f32x4 acc[MB][NT], sum_a[MB];
 #pragma unroll
@@ -223,11 +233,11 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
                 u32x4 raw[kRaw], part[kParts];
-                if constexpr (kAheadA && kWhole) {
+                if constexpr (kWhole) {
 #pragma unroll
-                    for (int r = 0; r < kRaw; ++r) raw[r] = a[q][r];
+                    for (int r = 0; r < kRaw; ++r) raw[r] = kAheadA ? a[kAheadA ? q : 0][r] : half_a[q & 1][b][r];
                 } else {
-                    load_eight<kWhole>(row[b], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, g.vec_a != 0, raw);
+                    load_eight<false>(row[b], (int64_t)kb * kTileK + 32 * q, g.K - 8 * h, g.vec_a != 0, raw);
                 }
                 operand<T>(raw, part);
 #pragma unroll
@@ -237,6 +247,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
                     for (int t = 0; t < NT; ++t) acc[b][t] = Q::mfma(part[p], bw[t], acc[b][t]);
                 }
             }
+            if (kWhole && (q & 1)) request_half(q == 1 ? (int64_t)kb * kTileK + 64 : (int64_t)next * kTileK);
             if (q % kSpan == kSpan - 1) {  // the end of a group
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -256,21 +267,22 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
 #pragma unroll
         for (int d = 0; d < kAhead; ++d) request(slots[d], last(k0 + d));
         request_a(ahead_a[0], k0);
+        request_half((int64_t)k0 * kTileK);
     }
-    constexpr int kTurn = kAhead < 2 ? 2 : kAhead;  // the two buffers of A take turns
-    for (int kb = k0; kb < kw; kb += kTurn) {
+    static_assert(kAhead == 2, "the two buffers of A take turns with the slots");
+    for (int kb = k0; kb < kw; kb += kAhead) {
 #pragma unroll
-        for (int d = 0; d < kTurn; ++d) {
+        for (int d = 0; d < kAhead; ++d) {
             if (kb + d >= kw) break;
-            request_a(ahead_a[(d + 1) & 1], last(kb + d + 1));
-            consume(slots[d % kAhead], ahead_a[d & 1], kb + d, Constant<1>{});
-            request(slots[d % kAhead], last(kb + d + kAhead));
+            request_a(ahead_a[d ^ 1], last(kb + d + 1));
+            consume(slots[d], ahead_a[d], kb + d, last(kb + d + 1), Constant<1>{});
+            request(slots[d], last(kb + d + kAhead));
         }
     }
 #pragma unroll 1
     for (int kb = kw; kb < k1; ++kb) {
         request(slots[0], kb);
-        consume(slots[0], ahead_a[0], kb, Constant<0>{});
+        consume(slots[0], ahead_a[0], kb, kb, Constant<0>{});
     }
 
     // Lane (h, c) holds rows 4 h .. 4 h + 3 of column c of each block.
@@ -304,8 +316,17 @@ cn_status launch_gemm(const GemmW4Args &g, hipStream_t st) {
 
 template <typename T, int GROUPS>
 cn_status run_gemm(const GemmW4Args &g, hipStream_t st) {
-    if (g.M > 32) return launch_gemm<T, GROUPS == 4 ? 1 : 2, 4, 8, GROUPS>(g, st);  // (two columns of groups of 32 would spill)
-    if (g.M > 16) return launch_gemm<T, 2, 2, 8, GROUPS>(g, st);
+    if (g.M > 16) {
+        // Two blocks of rows per workgroup (four: 64 rows of 8192 x 16384 in 78 us instead of 61), and four tiles of columns where that
+        // still makes a workgroup per compute unit: A comes from the L2 anew for every workgroup, and its lines are what bounds
+        // this (64 rows of 8192 x 16384 61 us, 91 with two tiles; of 8192 x 8192 32 and 48; 32 rows of it, which would be 128
+        // workgroups, 32 and 24).
+        const int64_t workgroups = (int64_t)(g.tiles_n / 4) * ((g.M + 31) / 32);
+        if constexpr (GROUPS < 4) {  // (four columns of groups of 32 would spill)
+            if (workgroups >= 256) return launch_gemm<T, 4, 2, 8, GROUPS>(g, st);
+        }
+        return launch_gemm<T, 2, 2, 8, GROUPS>(g, st);
+    }
     // Wide workgroups share A and its sums (one row of 16384 x 16384: 33.0 us, 38.3 us with narrow ones, 34.5 with four tiles of
     // columns, 34.0 with one tile of 128 rows ahead, 38.6 with four); narrow ones, with K among more wavefronts, fill the chip.
     if (g.tiles_n >= 512) return launch_gemm<T, 2, 1, 8, GROUPS>(g, st);
