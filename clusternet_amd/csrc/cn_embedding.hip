@@ -5,6 +5,7 @@
 // Lookup      out[t] = round(scale * E[tok[t]]).  Bound by memory: every row read once, every output written once.
 //
 // Gradient    dE[v] = scale * sum over {t : tok[t] = v} of dY[t], in fp32.
+//   Up to kDirectItems positions and rows that are not wide: see grad_direct_kernel.  Otherwise:
 //   1. The positions are sorted by token, stably, by a radix sort of my own digits: ceil(log2(rows + 1)) bits in as many
 //      passes as digits of at most kMaxDigit bits need (two for a table of up to 2^18 rows).  A token outside the table
 //      takes the key `rows` and so comes last.  Up to kSmallItems positions one workgroup does all passes in LDS; beyond,
@@ -300,6 +301,22 @@ __device__ __forceinline__ void finish_row(E *at, const float (&sum)[VEC], float
     }
 }
 
+// Zeros for the rows of dE from row0 on that are not named: this workgroup's slab of columns, 16 bytes a lane (one element where
+// rows are not made of whole vectors).
+template <typename E, int VEC>
+__device__ __forceinline__ void fill_unnamed(const GradArgs &a, const uint8_t *named, int64_t row0, E *__restrict__ de) {
+    constexpr int kPiece = VEC == 1 ? 1 : 16 / (int)sizeof(E);
+    const float zero[kPiece] = {};
+    const int64_t slab = (int64_t)blockIdx.y * a.lanes * VEC;
+    const int64_t width = a.cols - slab < (int64_t)a.lanes * VEC ? a.cols - slab : (int64_t)a.lanes * VEC;
+    const int pieces = (int)(width / kPiece);
+    const int per = pieces >= 256 ? 1 : 256 / pieces, sub = threadIdx.x / pieces < per ? threadIdx.x / pieces : -1;
+    for (int r = pieces >= 256 ? 0 : sub; r >= 0 && r < kZeroRows; r += per)
+        if (!named[r])
+            for (int x = pieces >= 256 ? threadIdx.x : threadIdx.x - sub * pieces; x < pieces; x += 256)
+                store_f32<kPiece, true>(de + (row0 + r) * a.lde + slab + (int64_t)x * kPiece, zero);
+}
+
 // UNIFORM: a wavefront's lanes share their chunk (64 lanes and more a row), so that keys and positions are scalar loads.
 template <typename T, typename E, int VEC, bool UNIFORM>
 __global__ __launch_bounds__(256) void grad_chunks_kernel(GradArgs a, const T *__restrict__ dy, E *__restrict__ de) {
@@ -316,17 +333,7 @@ __global__ __launch_bounds__(256) void grad_chunks_kernel(GradArgs a, const T *_
             named[threadIdx.x] = row >= a.rows || (lo < a.count && (int64_t)a.keys[lo] == row);
         }
         __syncthreads();
-        // this workgroup's slab of columns, 16 bytes a lane (one element where rows are not made of whole vectors)
-        constexpr int kPiece = VEC == 1 ? 1 : 16 / (int)sizeof(E);
-        const float zero[kPiece] = {};
-        const int64_t slab = (int64_t)blockIdx.y * a.lanes * VEC;
-        const int64_t width = a.cols - slab < (int64_t)a.lanes * VEC ? a.cols - slab : (int64_t)a.lanes * VEC;
-        const int pieces = (int)(width / kPiece);
-        const int per = pieces >= 256 ? 1 : 256 / pieces, sub = threadIdx.x / pieces < per ? threadIdx.x / pieces : -1;
-        for (int r = pieces >= 256 ? 0 : sub; r >= 0 && r < kZeroRows; r += per)
-            if (!named[r])
-                for (int x = pieces >= 256 ? threadIdx.x : threadIdx.x - sub * pieces; x < pieces; x += 256)
-                    store_f32<kPiece, true>(de + (row0 + r) * a.lde + slab + (int64_t)x * kPiece, zero);
+        fill_unnamed<E, VEC>(a, named, row0, de);
         return;
     }
     const int per = 256 / a.lanes, sub = threadIdx.x / a.lanes, lane = threadIdx.x - sub * a.lanes;
@@ -382,6 +389,100 @@ __global__ __launch_bounds__(256) void grad_chunks_kernel(GradArgs a, const T *_
         }
     }
     close(end < a.count && a.keys[end] == run);
+}
+
+// Few positions and rows that are not wide, in one launch and without sorting: workgroup t compares token t with all others.  If
+// an earlier one is the same it ends; else it has its list of positions, in order, from the ballots, its groups of lanes add
+// every per-th of them, and the groups' sums are added in order.  At most 32 lanes a row, so that per is 8 or more: even if all
+// positions name one row, no more than 256 are added one after the other, kDirectAhead in flight.  (128 windows of 11 words x
+// 120, fp32: 9.5 us, 19.9 by sorting; 2048 positions 9.5 and 21, all of them the same row 28.5 and 23.3.)  Every slab of
+// columns compares anew: two at most (four: 2048 x 1024 bf16 in 17 us, by sorting in 20, all the same row in 65 and 25).
+constexpr int kDirectItems = 2048, kDirectLanes = 32, kDirectSlabs = 2, kDirectAhead = 8;
+
+template <typename T, typename E, typename I, int VEC>
+__global__ __launch_bounds__(256) void grad_direct_kernel(GradArgs a, const I *__restrict__ tokens, const T *__restrict__ dy,
+                                                          E *__restrict__ de) {
+    __shared__ uint64_t words[kDirectItems / 64];
+    __shared__ uint16_t list[kDirectItems];
+    __shared__ float partial[256 * VEC];
+    __shared__ uint8_t named[kZeroRows];
+    const int n = (int)a.count, wave = threadIdx.x >> 6, lane64 = threadIdx.x & 63;
+    if ((int)blockIdx.x >= n) {  // zeros for the rows that no token names
+        const int64_t row0 = (int64_t)((int)blockIdx.x - n) * kZeroRows;
+        if (threadIdx.x < kZeroRows) named[threadIdx.x] = row0 + threadIdx.x >= a.rows;
+        __syncthreads();
+        for (int j = threadIdx.x; j < n; j += 256) {
+            const int64_t row = (int64_t)tokens[j];
+            if (row >= row0 && row < row0 + kZeroRows) named[row - row0] = 1;
+        }
+        __syncthreads();
+        fill_unnamed<E, VEC>(a, named, row0, de);
+        return;
+    }
+    const int t = (int)blockIdx.x;
+    const int64_t token = (int64_t)tokens[t];
+    if (token < 0 || token >= a.rows) return;
+    constexpr int kScans = kDirectItems / 256;
+    I other[kScans];
+#pragma unroll
+    for (int i = 0; i < kScans; ++i) {
+        const int j = (i * 4 + wave) * 64 + lane64;
+        other[i] = tokens[j < n ? j : n - 1];
+    }
+#pragma unroll
+    for (int i = 0; i < kScans; ++i) {
+        const int w = i * 4 + wave;
+        const uint64_t same = __ballot(w * 64 + lane64 < n && (int64_t)other[i] == token);
+        if (lane64 == 0) words[w] = same;
+    }
+    __syncthreads();
+    // every wavefront by itself; a lane has a word
+    uint64_t mine = lane64 < kDirectItems / 64 ? words[lane64] : 0u;
+    const uint64_t earlier = lane64 < t / 64 ? mine : lane64 == t / 64 ? mine & (((uint64_t)1 << (t & 63)) - 1) : 0u;
+    if (__ballot(earlier != 0)) return;  // the first of them does it
+    int upto = __popcll(mine);
+    for (int off = 1; off < 64; off <<= 1) {
+        const int before = __shfl_up(upto, off, 64);
+        if (lane64 >= off) upto += before;
+    }
+    const int matches = __shfl(upto, 63, 64);
+    if (wave == 0) {
+        int at = upto - __popcll(mine);
+        for (; mine; mine &= mine - 1) list[at++] = (uint16_t)(lane64 * 64 + __builtin_ctzll(mine));
+    }
+    __syncthreads();
+
+    const int per = 256 / a.lanes, sub = threadIdx.x / a.lanes, lane = threadIdx.x - sub * a.lanes;
+    const int64_t col = ((int64_t)blockIdx.y * a.lanes + lane) * VEC;
+    const bool in = col < a.cols;
+    float sum[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum[e] = 0.0f;
+    if (in) {
+        for (int r = sub; r < matches; r += per * kDirectAhead) {
+            float v[kDirectAhead][VEC];
+#pragma unroll
+            for (int j = 0; j < kDirectAhead; ++j)
+                if (r + j * per < matches) load_f32<VEC>(dy + (int64_t)list[r + j * per] * a.ldy + col, v[j]);
+#pragma unroll
+            for (int j = 0; j < kDirectAhead; ++j)
+                if (r + j * per < matches) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) sum[e] += v[j][e];
+                }
+        }
+    }
+    const int groups = matches < per ? matches : per;
+    if (groups > 1) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) partial[e * 256 + threadIdx.x] = sum[e];
+        __syncthreads();
+        if (sub == 0)
+            for (int g = 1; g < groups; ++g)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sum[e] += partial[e * 256 + g * a.lanes + lane];
+    }
+    if (sub == 0 && in) finish_row<VEC>(de + token * a.lde + col, sum, a.scale, a.accumulate != 0);
 }
 
 // The runs that cross chunk borders.  Workgroup c takes the run that begins in chunk c and goes on into the next, if there is
@@ -506,8 +607,9 @@ cn_status sort_tokens(const I *tokens, int64_t count, int64_t rows, const GradPl
 }
 
 template <typename T, typename E, int VEC>
-cn_status run_grad(GradArgs a, const void *dy, void *de, hipStream_t st) {
+cn_status run_grad(GradArgs a, const void *tokens, int token_bits, bool direct, const void *dy, void *de, hipStream_t st) {
     a.lanes = lanes_for(a.cols, VEC);
+    if (direct && a.lanes > kDirectLanes) a.lanes = kDirectLanes;
     const int64_t slabs = (a.cols + (int64_t)a.lanes * VEC - 1) / ((int64_t)a.lanes * VEC);
     const int per = 256 / a.lanes;
     a.chunk_blocks = (a.chunks + per - 1) / per;
@@ -518,6 +620,15 @@ cn_status run_grad(GradArgs a, const void *dy, void *de, hipStream_t st) {
         return CN_ERR_SHAPE;
     }
     if (a.chunk_blocks + zero_blocks == 0) return CN_OK;
+    if (direct) {
+        const dim3 grid((unsigned)(a.count + zero_blocks), (unsigned)slabs);
+        if (token_bits == 32)
+            hipLaunchKernelGGL((grad_direct_kernel<T, E, int32_t, VEC>), grid, dim3(256), 0, st, a, (const int32_t *)tokens, (const T *)dy, (E *)de);
+        else
+            hipLaunchKernelGGL((grad_direct_kernel<T, E, int64_t, VEC>), grid, dim3(256), 0, st, a, (const int64_t *)tokens, (const T *)dy, (E *)de);
+        CN_HIP(hipGetLastError());
+        return CN_OK;
+    }
     const dim3 grid((unsigned)(a.chunk_blocks + zero_blocks), (unsigned)slabs);
     if (a.lanes >= 64)
         hipLaunchKernelGGL((grad_chunks_kernel<T, E, VEC, true>), grid, dim3(256), 0, st, a, (const T *)dy, (E *)de);
@@ -617,8 +728,13 @@ cn_status cn_embedding_grad(const void *dy, int dy_dtype, int64_t ldy, const voi
     hipStream_t st = (hipStream_t)stream;
     const GradPlan p = plan_grad(count, rows, cols);
     GradSpace space = lay_out(workspace, p, count, cols);
+    // whole vectors: 16 bytes of dY; the parts and dE hold as many elements
+    const int64_t vec = 16 / (int64_t)dtype_bytes(dy_dtype);
+    const bool wide = cols % vec == 0 && ldy % vec == 0 && lde % vec == 0 && aligned_to(dy, 16) &&
+                      aligned_to(de, (size_t)vec * dtype_bytes(de_dtype));
+    const bool direct = count > 0 && count <= kDirectItems && cols <= kDirectSlabs * kDirectLanes * (wide ? vec : 1);
     int sorted = 0;
-    if (count > 0) {
+    if (count > 0 && !direct) {
         s = token_bits == 32 ? sort_tokens((const int32_t *)tokens, count, rows, p, space, &sorted, st)
                              : sort_tokens((const int64_t *)tokens, count, rows, p, space, &sorted, st);
         if (s != CN_OK) return s;
@@ -630,15 +746,12 @@ cn_status cn_embedding_grad(const void *dy, int dy_dtype, int64_t ldy, const voi
     a.count = count; a.rows = rows; a.cols = cols; a.ldy = ldy; a.lde = lde;
     a.chunks = p.chunks; a.chunk = p.chunk;
     a.scale = scale; a.accumulate = accumulate != 0;
-    // whole vectors: 16 bytes of dY; the parts and dE hold as many elements
-    const int64_t vec = 16 / (int64_t)dtype_bytes(dy_dtype);
-    const bool wide = cols % vec == 0 && ldy % vec == 0 && lde % vec == 0 && aligned_to(dy, 16) &&
-                      aligned_to(de, (size_t)vec * dtype_bytes(de_dtype));
     auto go = [&](auto in, auto to) -> cn_status {
         typedef decltype(in) T;
         typedef decltype(to) E;
         constexpr int kWide = 16 / (int)sizeof(T);
-        return wide ? run_grad<T, E, kWide>(a, dy, de, st) : run_grad<T, E, 1>(a, dy, de, st);
+        return wide ? run_grad<T, E, kWide>(a, tokens, token_bits, direct, dy, de, st)
+                    : run_grad<T, E, 1>(a, tokens, token_bits, direct, dy, de, st);
     };
     if (dy_dtype == CN_F32) return go(0.0f, 0.0f);
     if (dy_dtype == CN_F16) return de_dtype == CN_F32 ? go((f16_t)0, 0.0f) : go((f16_t)0, (f16_t)0);

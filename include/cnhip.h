@@ -362,7 +362,8 @@ cn_status cn_embedding(const void *table_device, int dtype, int64_t rows, int64_
                        int64_t ldo, void *stream);
 
 /* The gradient of cn_embedding with respect to its table, dE[v][:] = scale * sum of dY[t][:] over the t with
- * tokens[t] == v, summed in fp32 in an order that depends on the tokens and the sizes alone (the same bits every time).
+ * tokens[t] == v, summed in fp32 in an order that depends on the tokens, the
+ * sizes and the alignment alone (the same bits every time).
  * accumulate == 0: all rows x cols of dE are written, zeros where no token names the row;
  * accumulate != 0: the sums are added to dE, and rows that no token names are left as they are: with scale = -rate it is
  * the update of the reference's kUpdateVocabWithGradient.

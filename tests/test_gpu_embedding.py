@@ -134,7 +134,8 @@ def _check_grad(torch, dY, tokens, rows, scale, got, old=None):
 
 SIZES = [(1, 1, 1), (1, 3, 100), (7, 5, 3), (2, 16, 5000), (100002, 120, 1408), (513, 64, 8192), (513, 64, 8193),
          (300, 1001, 700), (3000, 33, 20000), (70000, 48, 70001), (600000, 8, 30000), (50, 4100, 333), (1000, 2048, 3000),
-         (511, 16, 9000), (512, 16, 9000), (4000, 4, 131072), (4000, 4, 131073), (2 ** 20, 2, 300001)]
+         (511, 16, 9000), (512, 16, 9000), (4000, 4, 131072), (4000, 4, 131073), (2 ** 20, 2, 300001),
+         (999, 64, 2047), (999, 256, 2048), (999, 260, 2048), (999, 256, 2049), (999, 64, 1025), (5000, 61, 2048), (40, 512, 2000)]
 
 
 @pytest.mark.parametrize("rows,cols,count", SIZES)
@@ -156,12 +157,13 @@ def test_gradient(torch, rows, cols, count, dtype, to, index):
     _check_grad(torch, dY, tokens, rows, -0.1, into, old)
 
 
-@pytest.mark.parametrize("count", [1, 7, 8, 9, 64, 65, 4097, 30001])
+@pytest.mark.parametrize("count", [1, 7, 8, 9, 64, 65, 2048, 2049, 4097, 30001])
 @pytest.mark.parametrize("which", ["one token", "two in turn", "all padded", "each its own", "descending"])
-def test_gradient_of_extreme_texts(torch, count, which):
+@pytest.mark.parametrize("cols", [24, 600])
+def test_gradient_of_extreme_texts(torch, count, which, cols):
     """Runs that fill every chunk, none, or exactly one; small whole numbers, so the sums are exact whatever their order."""
     import clusternet_amd as cn
-    rows, cols = 40000, 24
+    rows = 40000
     i = torch.arange(count, device="cuda")
     tokens = {"one token": i * 0 + 12345, "two in turn": (i % 2) * 39999, "all padded": i * 0 - 1, "each its own": (i * 7) % rows,
               "descending": rows - 1 - i % rows}[which].to(torch.int32)
