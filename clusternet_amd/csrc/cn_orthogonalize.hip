@@ -59,7 +59,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kUnit = 16384.0f, kPolyUnit = 1024.0f;  // the stored number for 1: of X, A and T, and of P and Q
 constexpr int kPad = 256;                           // rows and columns are padded to whole tiles
-constexpr int kStage = 32;                          // of k
 
 int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
 
