@@ -79,11 +79,6 @@ __device__ __forceinline__ void split_store(f16_t *m, size_t at, const float (&v
     *reinterpret_cast<f16x4 *>(m + at) = hi;
     *reinterpret_cast<f16x4 *>(m + at + 32) = lo;
 }
-__device__ __forceinline__ void split_load(const f16_t *m, size_t at, float (&v)[4]) {
-    const f16x4 hi = *reinterpret_cast<const f16x4 *>(m + at), lo = *reinterpret_cast<const f16x4 *>(m + at + 32);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)hi[e] + (float)lo[e];
-}
 
 // ---- the update whose direction is wanted ---------------------------------------------------------------------------------
 // G itself, or momentum and gradient of a training step.
@@ -97,21 +92,25 @@ struct Source {
     int64_t rows, cols;
 };
 
-// One element of the update.  `advance`: the momentum is moved on (once per step), else read as it is.
-template <typename T>
-__device__ __forceinline__ float update_of(const Source &s, int64_t r, int64_t c, bool advance) {
-    const float g = (float)((const T *)s.grad)[r * s.ldg + c];
-    if (!s.momentum) return g;
-    float *at = s.momentum + r * s.ldm + c;
-    float m = *at;
-    if (advance) {
-        m = s.mu * m + g;
-        *at = m;
+// VEC neighbouring elements of what the update is made of, and the update; `advance` moves the momentum on (once per step).
+template <int VEC> struct Pieces {
+    float g[VEC], m[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void load_pieces(const Source &s, int64_t r, int64_t c, Pieces<VEC> &p) {
+    load_f32<VEC>((const T *)s.grad + r * s.ldg + c, p.g);
+    if (s.momentum) load_f32<VEC>(s.momentum + r * s.ldm + c, p.m);
+}
+template <int VEC>
+__device__ __forceinline__ void update_of(const Source &s, Pieces<VEC> &p, bool advance, float (&u)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        if (advance && s.momentum) p.m[e] = s.mu * p.m[e] + p.g[e];
+        u[e] = !s.momentum ? p.g[e] : s.nesterov ? p.g[e] + s.mu * p.m[e] : p.m[e];
     }
-    return s.nesterov ? g + s.mu * m : m;
 }
 
-constexpr int kNormBlocks = 1024;
+constexpr int kNormBlocks = 2048, kNormRows = 8;
 
 __device__ __forceinline__ double block_sum(double v, double *scratch) {
 #pragma unroll
@@ -124,20 +123,27 @@ __device__ __forceinline__ double block_sum(double v, double *scratch) {
 }
 
 // Moves the momentum on and sums the squares of the update, in 64 bits (no overflow for any finite fp32), a part per workgroup.
-template <typename T>
+template <typename T, int VEC>
 __global__ __launch_bounds__(256) void norm_kernel(Source s, double *parts) {
     __shared__ double scratch[4];
     double sum = 0.0;
-    const int64_t tiles_c = (s.cols + 255) / 256;
-    for (int64_t t = blockIdx.x; t < tiles_c * ((s.rows + 15) / 16); t += gridDim.x) {
-        const int64_t r0 = t / tiles_c * 16, c = (t % tiles_c) * 256 + threadIdx.x;
+    const int64_t tiles_c = (s.cols + 256 * VEC - 1) / (256 * VEC);
+    for (int64_t t = blockIdx.x; t < tiles_c * ((s.rows + kNormRows - 1) / kNormRows); t += gridDim.x) {
+        const int64_t r0 = t / tiles_c * kNormRows, c = ((t % tiles_c) * 256 + threadIdx.x) * VEC;
         if (c >= s.cols) continue;
-#pragma unroll 8
-        for (int i = 0; i < 16; ++i)
-            if (r0 + i < s.rows) {
-                const double u = (double)update_of<T>(s, r0 + i, c, true);
-                sum += u * u;
-            }
+        Pieces<VEC> p[kNormRows];
+#pragma unroll
+        for (int i = 0; i < kNormRows; ++i)
+            if (r0 + i < s.rows) load_pieces<T, VEC>(s, r0 + i, c, p[i]);
+#pragma unroll
+        for (int i = 0; i < kNormRows; ++i) {
+            if (r0 + i >= s.rows) break;
+            float u[VEC];
+            update_of<VEC>(s, p[i], true, u);
+            if (s.momentum) store_f32<VEC>(s.momentum + (r0 + i) * s.ldm + c, p[i].m);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum += (double)u[e] * (double)u[e];
+        }
     }
     sum = block_sum(sum, scratch);
     if (threadIdx.x == 0) parts[blockIdx.x] = sum;
@@ -146,11 +152,29 @@ __global__ __launch_bounds__(256) void norm_kernel(Source s, double *parts) {
 // X0 in both orientations, zeros in the padding.  A workgroup takes 64 x 64 elements of X (m x n).  `exact` (a gradient of 16
 // bits): only the power of two of the scale is applied, so that the stored numbers are the gradient's own, hi alone; the rest,
 // r in [1, 2), goes to the products of X0: factors = 1, r, r r.
-template <typename T>
+template <typename T, int VEC>
 __global__ __launch_bounds__(256) void split_kernel(Source s, const double *parts, int part_count, int flip, int exact, int64_t mp,
                                                     int64_t np, f16_t *x, f16_t *xt, float *factors) {
     __shared__ double scratch[4];
     __shared__ float tile[64][65];
+    const int64_t blocks_n = np / 64;
+    const int64_t i0 = blockIdx.x / blocks_n * 64, j0 = blockIdx.x % blocks_n * 64;  // of X
+    // read along the rows of G, whichever way it lies
+    const int64_t r0 = flip ? j0 : i0, c0 = flip ? i0 : j0;
+    constexpr int kLanes = 64 / VEC, kReads = 64 * kLanes / 256;
+    const int read_row = threadIdx.x / kLanes, read_col = threadIdx.x % kLanes * VEC;
+    float u[kReads][VEC];
+#pragma unroll
+    for (int q = 0; q < kReads; ++q) {
+        const int64_t r = r0 + read_row + q * (256 / kLanes), c = c0 + read_col;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) u[q][e] = 0.0f;
+        if (r < s.rows && c < s.cols) {
+            Pieces<VEC> p;
+            load_pieces<T, VEC>(s, r, c, p);
+            update_of<VEC>(s, p, false, u[q]);
+        }
+    }
     double sum = 0.0;
     for (int i = threadIdx.x; i < part_count; i += 256) sum += parts[i];
     sum = block_sum(sum, scratch);
@@ -166,17 +190,14 @@ __global__ __launch_bounds__(256) void split_kernel(Source s, const double *part
         factors[1] = rest;
         factors[2] = rest * rest;
     }
-    const int64_t blocks_n = np / 64;
-    const int64_t i0 = blockIdx.x / blocks_n * 64, j0 = blockIdx.x % blocks_n * 64;  // of X
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 8
-    for (int q = 0; q < 16; ++q) {
-        const int a = wave + 4 * q;
-        // read along the rows of G, whichever way it lies
-        const int64_t r = (flip ? j0 : i0) + a, c = (flip ? i0 : j0) + lane;
-        const float v = r < s.rows && c < s.cols ? (float)((double)update_of<T>(s, r, c, false) * to_unit) : 0.0f;
-        if (flip) tile[lane][a] = v; else tile[a][lane] = v;
-    }
+#pragma unroll
+    for (int q = 0; q < kReads; ++q)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int a = read_row + q * (256 / kLanes), b = read_col + e;
+            const float v = (float)((double)u[q][e] * to_unit);
+            if (flip) tile[b][a] = v; else tile[a][b] = v;
+        }
     __syncthreads();
     const int row = threadIdx.x >> 4, col = (threadIdx.x & 15) * 4;
 #pragma unroll
@@ -886,12 +907,19 @@ constexpr int kFirstGroup = 3, kGroup = 2;  // steps
 
 template <typename T>
 cn_status newton_schulz(const Source &src, int steps, const Result &res, const Sizes &z, const Space &s, int device, hipStream_t st) {
-    const int64_t norm_tiles = ((src.cols + 255) / 256) * ((src.rows + 15) / 16);
-    const int norm_blocks = (int)(norm_tiles < kNormBlocks ? norm_tiles : kNormBlocks);
     const int exact = sizeof(T) == 2 && !src.momentum;
-    hipLaunchKernelGGL((norm_kernel<T>), dim3(norm_blocks), dim3(256), 0, st, src, s.norms);
-    hipLaunchKernelGGL((split_kernel<T>), dim3((unsigned)((z.mp / 64) * (z.np / 64))), dim3(256), 0, st, src, s.norms, norm_blocks, z.flip,
-                       exact, z.mp, z.np, s.x, s.xt[0], s.factors);
+    int norm_blocks = 0;
+    auto begin = [&](auto vector) {
+        constexpr int VEC = decltype(vector)::value;
+        const int64_t tiles = ((src.cols + 256 * VEC - 1) / (256 * VEC)) * ((src.rows + kNormRows - 1) / kNormRows);
+        norm_blocks = (int)(tiles < kNormBlocks ? tiles : kNormBlocks);
+        hipLaunchKernelGGL((norm_kernel<T, VEC>), dim3(norm_blocks), dim3(256), 0, st, src, s.norms);
+        hipLaunchKernelGGL((split_kernel<T, VEC>), dim3((unsigned)((z.mp / 64) * (z.np / 64))), dim3(256), 0, st, src, s.norms, norm_blocks,
+                           z.flip, exact, z.mp, z.np, s.x, s.xt[0], s.factors);
+    };
+    const bool wide = src.cols % 4 == 0 && src.ldg % 4 == 0 && aligned_to(src.grad, 4 * sizeof(T)) &&
+                      (!src.momentum || (src.ldm % 4 == 0 && aligned_to(src.momentum, 16)));
+    if (wide) begin(Constant<4>{}); else begin(Constant<1>{});
     CN_HIP(hipGetLastError());
     Product base{};
     base.parts = s.parts;
