@@ -47,6 +47,9 @@ inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintp
 inline size_t dtype_bytes(int dtype) { return dtype == CN_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == CN_F32 || dtype == CN_F16 || dtype == CN_BF16; }
 
+// A launch has fewer than 2^32 work items in x and 2^16 workgroups in y.
+inline bool launchable(int64_t blocks, int threads, int64_t slabs = 1) { return blocks <= 0xffffffffLL / threads && slabs <= 65535; }
+
 // Device memory a caller hands over, dealt out in 256-byte steps.
 struct Carver {
     char *base;

@@ -615,10 +615,6 @@ cn_status run_grad(GradArgs a, const void *tokens, int token_bits, bool direct, 
     a.chunk_blocks = (a.chunks + per - 1) / per;
     const int64_t zero_blocks = a.accumulate ? 0 : (a.rows + kZeroRows - 1) / kZeroRows;
     const int64_t join_slabs = (a.cols + 64 * VEC - 1) / (64 * VEC);
-    if (a.chunk_blocks + zero_blocks > 0x7fffffffLL || slabs > 65535 || join_slabs > 65535) {
-        set_error("embedding_grad: too many rows or columns for one launch");
-        return CN_ERR_SHAPE;
-    }
     if (a.chunk_blocks + zero_blocks == 0) return CN_OK;
     if (direct) {
         const dim3 grid((unsigned)(a.count + zero_blocks), (unsigned)slabs);
@@ -646,10 +642,6 @@ cn_status run_lookup(const void *table, int64_t rows, int64_t cols, int64_t ld, 
     const int lanes = lanes_for(cols, VEC);
     const int64_t per = (int64_t)(256 / lanes) * kRowsAhead;
     const int64_t blocks = (count + per - 1) / per, slabs = (cols + (int64_t)lanes * VEC - 1) / ((int64_t)lanes * VEC);
-    if (blocks > 0x7fffffffLL || slabs > 65535) {
-        set_error("embedding: too many tokens or columns for one launch");
-        return CN_ERR_SHAPE;
-    }
     const dim3 grid((unsigned)blocks, (unsigned)slabs);
     if (bits == 32)
         hipLaunchKernelGGL((embedding_kernel<T, int32_t, VEC>), grid, dim3(256), 0, st, (const T *)table, rows, cols, ld,
@@ -685,11 +677,17 @@ cn_status cn_embedding(const void *table, int dtype, int64_t rows, int64_t cols,
     if (ldo < cols) { set_error("embedding: leading dimension too small"); return CN_ERR_SHAPE; }
     if (count == 0 || cols == 0) return CN_OK;
     if ((rows > 0 && !table) || !tokens || !out) { set_error("embedding: NULL pointer"); return CN_ERR_NULL; }
+    if (table == out) { set_error("embedding: the output is the table"); return CN_ERR_ARG; }
+    const int64_t vec = 16 / (int64_t)dtype_bytes(dtype);
+    const bool wide = cols % vec == 0 && ld % vec == 0 && ldo % vec == 0 && aligned_to(table, 16) && aligned_to(out, 16);
+    const int64_t lanes = lanes_for(cols, wide ? vec : 1), per = 256 / lanes * kRowsAhead;
+    if (!launchable((count + per - 1) / per, 256, cols / (lanes * (wide ? vec : 1)) + 1)) {
+        set_error("embedding: too many tokens or columns for one launch");
+        return CN_ERR_SHAPE;
+    }
     Context *ctx;
     s = current_context(&ctx);
     if (s != CN_OK) return s;
-    const int64_t vec = 16 / (int64_t)dtype_bytes(dtype);
-    const bool wide = cols % vec == 0 && ld % vec == 0 && ldo % vec == 0 && aligned_to(table, 16) && aligned_to(out, 16);
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto zero) -> cn_status {
         typedef decltype(zero) T;
@@ -722,11 +720,17 @@ cn_status cn_embedding_grad(const void *dy, int dy_dtype, int64_t ldy, const voi
         return CN_ERR_WORKSPACE;
     }
     if (count > 0 && !aligned_to(workspace, 256)) { set_error("embedding_grad: the workspace is not aligned to 256 bytes"); return CN_ERR_ARG; }
+    if (count > 0 && de == dy) { set_error("embedding_grad: the gradient is the errors"); return CN_ERR_ARG; }
+    const GradPlan p = plan_grad(count, rows, cols);
+    const int64_t most = (p.chunks < kDirectItems ? kDirectItems : p.chunks) + (accumulate ? 0 : rows / kZeroRows + 1);
+    if (!launchable(most, 256, cols / 64 + 1)) {
+        set_error("embedding_grad: too many rows or columns for one launch");
+        return CN_ERR_SHAPE;
+    }
     Context *ctx;
     s = current_context(&ctx);
     if (s != CN_OK) return s;
     hipStream_t st = (hipStream_t)stream;
-    const GradPlan p = plan_grad(count, rows, cols);
     GradSpace space = lay_out(workspace, p, count, cols);
     // whole vectors: 16 bytes of dY; the parts and dE hold as many elements
     const int64_t vec = 16 / (int64_t)dtype_bytes(dy_dtype);

@@ -1017,6 +1017,10 @@ cn_status start(const char *what, const Source &src, int grad_dtype, int steps, 
         return CN_ERR_WORKSPACE;
     }
     if (!aligned_to(workspace, 256)) { set_error("%s: the workspace is not aligned to 256 bytes", what); return CN_ERR_ARG; }
+    if (src.momentum && (src.momentum == src.grad || src.momentum == res.out || src.grad == res.out)) {
+        set_error("%s: momentum, gradient and weights are not three matrices", what);
+        return CN_ERR_ARG;
+    }
     Context *ctx;
     const cn_status status = current_context(&ctx);
     if (status != CN_OK) return status;

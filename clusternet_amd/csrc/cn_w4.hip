@@ -507,7 +507,7 @@ QuantArgs quant_args(int64_t K, int64_t N, int64_t ld, int group, int columns) {
 cn_status check_weights(const char *what, int64_t K, int64_t N, int group) {
     if (K < 0 || N < 0) { set_error("%s: negative dimension", what); return CN_ERR_SHAPE; }
     if (group != 32 && group != 64 && group != 128) { set_error("%s: groups of %d rows (32, 64 or 128)", what, group); return CN_ERR_ARG; }
-    if (K > 0x7fffffffLL || N > 0x7fffffffLL || tiles_k_of(K) * ((N + 63) / 64) > 0x7fffffffLL) {
+    if (K > 0x7fffffffLL || N > 0x7fffffffLL || !launchable(tiles_k_of(K) * ((N + 63) / 64), 256)) {
         set_error("%s: too many weights for one launch", what);
         return CN_ERR_SHAPE;
     }
@@ -600,6 +600,8 @@ cn_status cn_gemm_w4(int64_t M, int64_t N, int64_t K, const void *A, int dtype, 
     if (M == 0 || N == 0) return CN_OK;
     if (!out || (K > 0 && (!A || !codes || !scales))) { set_error("gemm_w4: NULL pointer"); return CN_ERR_NULL; }
     if (!aligned_to(codes, 16)) { set_error("gemm_w4: the codes are not aligned to 16 bytes"); return CN_ERR_ARG; }
+    if (out == A) { set_error("gemm_w4: the output is A"); return CN_ERR_ARG; }
+    if (!launchable(tiles_n_of(N) / 2 + 1, 512)) { set_error("gemm_w4: too many columns for one launch"); return CN_ERR_SHAPE; }
     Context *ctx;
     s = current_context(&ctx);
     if (s != CN_OK) return s;

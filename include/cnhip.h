@@ -316,7 +316,7 @@ cn_status cn_dequantize_4bit(const int32_t *codes_device, const float *scales_de
 
 /* out (M x N) = A (M x K) W with W in that form; A and out of `dtype`.  Products are exact, sums and scales fp32, a
  * 16-bit result is rounded once.  Made for answers (a row per token, up to a few dozen); any M is right, but from a few
- * hundred rows on decoded weights are faster.  The same bits every time; needs no workspace.  A row of A with a number
+ * hundred rows on decoded weights are faster.  The same bits every time; needs no workspace.  out must not overlap A.  A row of A with a number
  * that is not finite gives NaNs.  The 8-bit relative is cn_gemm_f32_w8. */
 cn_status cn_gemm_w4(int64_t M, int64_t N, int64_t K, const void *A_device, int dtype, int64_t lda,
                      const int32_t *codes_device, const float *scales_device, const uint8_t *zeros_device, int group,
@@ -330,9 +330,9 @@ cn_status cn_gemm_w4(int64_t M, int64_t N, int64_t K, const void *A_device, int 
 
 /* out = the gradient with its singular values moved towards one: X = G / (|G|_F + 1e-7), transposed if rows > cols, then
  * `steps` times A = X X^T, X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X (five steps bring singular values from 0.002 to 1 of
- * the largest to between about 0.7 and 1.2).  To the accuracy of fp32 products, rounded once.  G and out are rows x cols,
- * CN_F32, CN_F16 or CN_BF16 each; out may be G.  A zero G gives zeros, one that is
- * not finite NaNs. */
+ * the largest to between about 0.7 and 1.2).  To the accuracy of fp32 products, rounded once; elements of X0 below 2^-38 count as
+ * zero (so does a gradient whose norm is that far below 1e-7).  G and out are rows x cols, CN_F32, CN_F16 or CN_BF16 each; out
+ * may be G.  A zero G gives zeros, one that is not finite NaNs. */
 size_t cn_orthogonalize_workspace_bytes(int64_t rows, int64_t cols);
 cn_status cn_orthogonalize(const void *G_device, int dtype, int64_t rows, int64_t cols, int64_t ldg, int steps,
                            void *out_device, int out_dtype, int64_t ldo, void *workspace_device,
@@ -342,7 +342,7 @@ cn_status cn_orthogonalize(const void *G_device, int dtype, int64_t rows, int64_
  *   momentum = momentum_factor * momentum + grad
  *   u        = nesterov ? grad + momentum_factor * momentum : momentum
  *   w        = (1 - learning_rate * weight_decay) * w - learning_rate * orthogonalize(u)
- * momentum and w fp32, the gradient of grad_dtype; every operation rounded to fp32.  A factor for the shape
+ * momentum and w fp32, the gradient of grad_dtype, none of them overlapping another; every operation rounded to fp32.  A factor for the shape
  * (such as sqrt(max(1, rows / cols))) is the caller's, in the rate. */
 cn_status cn_muon_update(float *momentum_device, int64_t ldm, const void *grad_device, int grad_dtype, int64_t ldg,
                          float *w_device, int64_t ldw, int64_t rows, int64_t cols, float momentum_factor,
@@ -356,14 +356,14 @@ cn_status cn_muon_update(float *momentum_device, int64_t ldm, const void *grad_d
  * Tokens are int32 (token_bits 32) or int64 (64) row numbers; a token outside [0, rows) names no row (padding). */
 
 /* out[t][:] = scale * table[tokens[t]][:], rounded once to the table's type; zeros where the token names no row.
- * table: rows x cols of `dtype` (CN_F32, CN_F16, CN_BF16), leading dimension ld; out: count x cols, ldo. */
+ * table: rows x cols of `dtype` (CN_F32, CN_F16, CN_BF16), leading dimension ld; out: count x cols, ldo, not overlapping it. */
 cn_status cn_embedding(const void *table_device, int dtype, int64_t rows, int64_t cols, int64_t ld,
                        const void *tokens_device, int token_bits, int64_t count, float scale, void *out_device,
                        int64_t ldo, void *stream);
 
 /* The gradient of cn_embedding with respect to its table, dE[v][:] = scale * sum of dY[t][:] over the t with
- * tokens[t] == v, summed in fp32 in an order that depends on the tokens, the
- * sizes and the alignment alone (the same bits every time).
+ * tokens[t] == v, summed in fp32 in an order that depends on the tokens, the sizes and the alignment alone (the same bits
+ * every time).
  * accumulate == 0: all rows x cols of dE are written, zeros where no token names the row;
  * accumulate != 0: the sums are added to dE, and rows that no token names are left as they are: with scale = -rate it is
  * the update of the reference's kUpdateVocabWithGradient.

@@ -154,6 +154,12 @@ def test_zero_and_not_finite(torch):
         G = _gradient(torch, 40, 70, 1)
         G[7, 9] = bad
         assert bool(cn.orthogonalize(G).isnan().all())
+    for dtype, rows, cols in ((torch.bfloat16, 40, 70), (torch.float16, 300, 2000), (torch.float32, 3000, 400), (torch.bfloat16, 3000, 400)):
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            G = _gradient(torch, rows, cols, 2).to(dtype)
+            G[rows - 1, cols - 1] = bad
+            assert bool(cn.orthogonalize(G).isnan().all())
+        assert not cn.orthogonalize(torch.zeros(rows, cols, device="cuda", dtype=dtype)).any()
     assert cn.orthogonalize(torch.empty(0, 5, device="cuda")).shape == (0, 5)
     assert cn.orthogonalize(torch.empty(5, 0, device="cuda")).shape == (5, 0)
 

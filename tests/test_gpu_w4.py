@@ -136,6 +136,21 @@ def test_quantisation_of_a_part_of_a_matrix(torch):
     assert bool((back == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype,K,N", [("float32", 16500, 4100), ("bfloat16", 16500, 8200), ("float16", 8300, 16400)])
+def test_weights_larger_than_the_caches(torch, dtype, K, N):
+    """What the small sizes hold to the definition, at a size that is written past the caches: the same numbers as from 128
+    rows at a time."""
+    import clusternet_amd as cn
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    W = (0.05 * torch.randn(K, N, device="cuda", generator=gen)).to(getattr(torch, dtype))
+    for zero_points in (False, True):
+        whole = cn.dequantize_4bit(cn.quantize_4bit(W, 64, zero_points), dtype=W.dtype)
+        for first in (0, 128, K // 256 * 128, K // 128 * 128):
+            part = W[first:first + 128].contiguous()
+            assert torch.equal(whole[first:first + 128], cn.dequantize_4bit(cn.quantize_4bit(part, 64, zero_points), dtype=W.dtype))
+        assert bool((whole.float() - W.float()).abs().max() <= 0.05)  # steps of a seventh of up to 0.35
+
+
 def _weights(torch, rng, K, N, group, zero_points, whole):
     import clusternet_amd as cn
     groups = -(-K // group)
@@ -150,7 +165,8 @@ def _weights(torch, rng, K, N, group, zero_points, whole):
 
 
 SIZES = [(1, 1, 1), (1, 128, 16), (1, 5, 33), (3, 127, 15), (16, 128, 64), (17, 130, 70), (13, 500, 199), (1, 4096, 1024), (33, 260, 48),
-         (64, 1000, 130), (65, 384, 100), (200, 129, 17), (2, 1056, 16400), (5, 200, 33000)]
+         (64, 1000, 130), (65, 384, 100), (200, 129, 17), (2, 1056, 16400), (5, 200, 33000), (20, 264, 16390),
+         (40, 390, 8210), (300, 136, 1650)]
 
 
 @pytest.mark.parametrize("M,K,N", SIZES)

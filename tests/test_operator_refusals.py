@@ -27,6 +27,10 @@ def test_embedding_refuses():
     _refused(f(AT, 0, 4, 4, 4, None, 32, 4, 1.0, AT, 4, None), NULL)
     _refused(f(AT, 0, 4, 4, 4, AT, 32, 4, 1.0, None, 4, None), NULL)
     assert f(None, 0, 0, 4, 4, None, 32, 0, 1.0, None, 4, None) == 0     # no tokens: nothing to do
+    _refused(f(AT, 0, 4, 4, 4, AT, 32, 4, 1.0, AT, 4, None), ARG)        # into the table itself
+    # more workgroups than a launch may have
+    _refused(f(AT, 0, 4, 2048, 2048, AT, 32, 2 ** 27, 1.0, 2 * AT, 2048, None), SHAPE)
+    _refused(f(AT, 0, 4, 2 ** 26 + 1, 2 ** 27, AT, 32, 4, 1.0, 2 * AT, 2 ** 27, None), SHAPE)
 
 
 def test_embedding_grad_refuses():
@@ -56,6 +60,10 @@ def test_embedding_grad_refuses():
     _refused(call(_14=size - 1), WORKSPACE)
     _refused(call(_13=AT + 16), ARG)          # alignment of the workspace
     assert call(_5=0, _9=1, _0=None, _3=None, _13=None, _14=0) == 0
+    _refused(call(), ARG)                     # onto the errors
+    big = need(100, 2 ** 30, 8)
+    _refused(call(_10=2 * AT, _6=2 ** 30, _14=big), SHAPE)             # 2^25 workgroups that write zeros
+    _refused(call(_10=2 * AT, _9=1, _7=2 ** 22 + 64, _2=2 ** 23, _12=2 ** 23, _14=2 ** 62), SHAPE)
 
 
 def test_binding_refuses_tensors_of_the_host():
@@ -113,6 +121,8 @@ def test_muon_update_refuses():
     for place in ("_0", "_2", "_5", "_14"):
         _refused(call(**{place: None}), NULL)
     _refused(call(_15=size - 1), WORKSPACE)
+    for places in ({}, {"_0": 2 * AT}, {"_2": 2 * AT}, {"_5": 2 * AT}):  # two or all of them the same matrix
+        _refused(call(**places), ARG)
     assert call(_8=0, _0=None, _2=None, _5=None, _14=None) == 0
 
 
@@ -159,6 +169,8 @@ def test_w4_refuses():
     for place in ("_3", "_6", "_7", "_10"):
         _refused(g(**{place: None}), NULL)
     _refused(g(_6=AT + 8), ARG)
+    _refused(g(), ARG)                        # the output is A
+    _refused(g(_10=2 * AT, _1=2 ** 30, _11=2 ** 30), SHAPE)
     assert g(_0=0, _3=None, _6=None, _7=None, _10=None) == 0
 
 
