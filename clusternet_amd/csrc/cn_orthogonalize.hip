@@ -22,9 +22,9 @@
 // 3 m^2 n + (4 g - 3) m^3 in place of g (3 m^2 n + m^3), at n = 4 m 42 % less for five steps as three and two.  A is computed from X
 // again after at most three steps in the beginning, where singular values grow, and two later on: with five steps in one group,
 // or three behind two, errors grow tenfold (emulated in 64 bits on Gaussian, orthogonal, rank-one, nearly low-rank spectra and
-// power laws), with three and two they stay at those of plain fp32.  Measured, steps alone -> in groups: 4096 x 16384 10.7 -> 6.8 ms,
-// 1000 x 4001 395 -> 342 us; equal by count at m = n, where it would only add launches.  Taken where the products' estimated
-// times add up to less (sizes_of).
+// power laws), with three and two they stay at those of plain fp32.  Measured, steps alone -> in groups: 4096 x 16384 bf16
+// 10.8 -> 6.65 ms, 1000 x 4001 384 -> 319 us, 1000 x 2000 283 -> 272, but 784 x 1024 186 -> 215 and 4096 x 4096 3.91 -> 4.27 ms:
+// taken where the products' estimated times add up to less (sizes_of; at twelve sizes at most 3 % off the better form).
 //
 // A gradient of 16 bits is its own hi if only the power of two of the scale is applied to it, so X0 X0^T is one product and Q X0
 // two, with nothing lost; the rest of the scale, in [1, 2), goes to their results (split_kernel).  (One product in place of
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
     // operands are read from LDS while the group before it computes, the first group's of a stage behind the barrier that
     // publishes it, which sits before the last group of the stage before.  (With all of a step's reads in front of its
     // instructions the wavefronts, in step after the barrier, took turns between LDS and matrix cores: 4400 cycles a stage
-    // of 256 x 256 x 32 instead of 3072.)
+    // of 256 x 256 x 32 instead of the 3100 that they compute.)
     constexpr int kGroups = kSteps * S::FM;
     static_assert(S::KS > 1 || kGroups % 2 == 0, "the buffers alternate across stages");
     f16x8 uh[2], ul[2], vh[2][S::FN], vl[2][S::FN];
