@@ -617,6 +617,13 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
             for (int n = 0; n < S::FN; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[mi][n][r] = 0.0f;
+        constexpr int kBlocks = S::FM * S::FN, kMine = (kBlocks + S::KS - 1) / S::KS;  // that a wavefront finishes
+        const int from = share * kMine, until = from + kMine < kBlocks ? from + kMine : kBlocks;
+        auto place_i = [&](int b) { return (int64_t)at.ti * TILE + (wave_i * S::FM + b / S::FN) * 32; };
+        auto place_j = [&](int b) { return (int64_t)at.tj * TILE + (wave_j * S::FN + b % S::FN) * 32; };
+        const bool finishes = at.slot < 0 && from < until;
+        Old old, next;
+        if (S::KS == 2 && finishes) load_old<FINISH>(g, g.old, place_i(from), place_j(from), old);  // on its way during the stages
         for (; at.stage < at.end; ++at.stage) {
             if constexpr (S::KS == 1) {
 #pragma unroll
@@ -650,7 +657,6 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
         }
         counted = false;
         float *own = reinterpret_cast<float *>(smem + S::DEPTH * 2 * kOperand) + wave * 1024;
-        constexpr int kBlocks = S::FM * S::FN, kMine = (kBlocks + S::KS - 1) / S::KS;
         if constexpr (S::KS == 2) {
             // the two halves meet: each wavefront of a pair takes half of their blocks (the first one a single block)
             const float *theirs = own + (share ? -1 : 1) * (S::WM * S::WN * 1024);
@@ -684,14 +690,10 @@ __global__ __launch_bounds__(threads_of<TILE>(), 1) void product_kernel(Product 
         }
         // a finished block, or its part of the sum as the registers lie: [32 x 32 block][number / 4][lane][4]
         const bool mirror = !(g.triangle && at.ti == at.tj);
-        auto place_i = [&](int b) { return (int64_t)at.ti * TILE + (wave_i * S::FM + b / S::FN) * 32; };
-        auto place_j = [&](int b) { return (int64_t)at.tj * TILE + (wave_j * S::FN + b % S::FN) * 32; };
-        const int from = share * kMine, until = from + kMine < kBlocks ? from + kMine : kBlocks;
         // One copy of the code for all blocks (unrolled it would be most of the kernel, fetched anew by every launch): the block's
         // registers are picked by a branch.  Old values are requested a block ahead, in front of the stores of the block before:
         // the counter that a load is waited for with would otherwise drain them first.
-        Old old, next;
-        if (at.slot < 0 && from < until) load_old<FINISH>(g, g.old, place_i(from), place_j(from), old);
+        if (S::KS == 1 && finishes) load_old<FINISH>(g, g.old, place_i(from), place_j(from), old);
 #pragma unroll 1
         for (int b = from; b < until; ++b) {
             f32x16 sum;
