@@ -590,7 +590,7 @@ def embedding(table, tokens, scale=1.0, out=None):
     rows, cols = table.shape
     count = tokens.numel()
     if out is None:
-        out = torch.empty(tokens.shape + (cols,), dtype=table.dtype, device=table.device)
+        out = table.new_empty((*tokens.shape, cols))
         ldo = cols
     else:
         if _dtype_code(out, "out", table.device) != code:
@@ -627,9 +627,9 @@ def embedding_grad(dY, tokens, rows, scale=1.0, out=None, out_dtype=None, accumu
         raise CnError(2, "Matrix size error: out %s, gradient %dx%d" % (tuple(out.shape), rows, cols))
     L = lib()
     size = L.cn_embedding_grad_workspace_bytes(count, rows, cols)
-    space = torch.empty(size, dtype=torch.uint8, device=dY.device)
+    space = dY.new_empty(size, dtype=torch.uint8) if size else None
     _run(L.cn_embedding_grad, dY.device, dY.data_ptr(), code, _ld(dY), tokens.data_ptr(), bits, count, rows, cols, scale,
-         int(accumulate), out.data_ptr(), out_code, _ld(out), space.data_ptr(), size)
+         1 if accumulate else 0, out.data_ptr(), out_code, _ld(out), space.data_ptr() if size else None, size)
     return out
 
 
@@ -734,7 +734,7 @@ def gemm_w4(A, W, out=None):
     if W.codes.device != device:
         raise ValueError("W is on %s, A on %s" % (W.codes.device, device))
     if out is None:
-        out = torch.empty((M, W.outer), dtype=A.dtype, device=device)
+        out = A.new_empty((M, W.outer))
     elif _dtype_code(out, "out", device) != code:
         raise TypeError("out must be of A's dtype %s" % A.dtype)
     if K != W.inner or out.shape[0] != M or out.shape[1] != W.outer:

@@ -395,8 +395,9 @@ __global__ __launch_bounds__(256) void grad_chunks_kernel(GradArgs a, const T *_
 // an earlier one is the same it ends; else it has its list of positions, in order, from the ballots, its groups of lanes add
 // every per-th of them, and the groups' sums are added in order.  At most 32 lanes a row, so that per is 8 or more: even if all
 // positions name one row, no more than 256 are added one after the other, kDirectAhead in flight.  (128 windows of 11 words x
-// 120, fp32: 9.5 us, 19.9 by sorting; 2048 positions 9.5 and 21, all of them the same row 28.5 and 23.3.)  Every slab of
-// columns compares anew: two at most (four: 2048 x 1024 bf16 in 17 us, by sorting in 20, all the same row in 65 and 25).
+// 120, fp32: 7.6 us, 19.9 by sorting; 2048 positions 8 and 21, all of them the same row 28.5 and 23.3.)  Every slab of
+// columns compares anew: two at most (four: 2048 x 1024 bf16 in 17 us, by sorting in 20, all the same row in 65 and 25).  Rows of
+// up to 256 elements always go this way, so that such calls need no workspace; wider ones where 16 bytes a lane cover them in two.
 constexpr int kDirectItems = 2048, kDirectLanes = 32, kDirectSlabs = 2, kDirectAhead = 8;
 
 template <typename T, typename E, typename I, int VEC>
@@ -560,6 +561,9 @@ GradPlan plan_grad(int64_t count, int64_t rows, int64_t cols) {
     return p;
 }
 
+// Whatever the type and the alignment: such calls need no workspace.
+bool never_sorted(int64_t count, int64_t cols) { return count > 0 && count <= kDirectItems && cols <= kDirectSlabs * kDirectLanes * 4; }
+
 struct GradSpace {
     uint32_t *keys[2], *positions[2], *counts, *totals;
     float *parts;
@@ -700,7 +704,7 @@ cn_status cn_embedding(const void *table, int dtype, int64_t rows, int64_t cols,
 
 size_t cn_embedding_grad_workspace_bytes(int64_t count, int64_t rows, int64_t cols) {
     if (count <= 0 || rows < 0 || cols <= 0 || count > 0x7fffffffLL || rows > 0x7fffffffLL) return 0;
-    return lay_out(nullptr, plan_grad(count, rows, cols), count, cols).bytes;
+    return never_sorted(count, cols) ? 0 : lay_out(nullptr, plan_grad(count, rows, cols), count, cols).bytes;
 }
 
 cn_status cn_embedding_grad(const void *dy, int dy_dtype, int64_t ldy, const void *tokens, int token_bits, int64_t count,
@@ -714,12 +718,13 @@ cn_status cn_embedding_grad(const void *dy, int dy_dtype, int64_t ldy, const voi
     if (s != CN_OK) return s;
     if (ldy < cols) { set_error("embedding_grad: leading dimension too small"); return CN_ERR_SHAPE; }
     if (rows == 0 || cols == 0 || (accumulate && count == 0)) return CN_OK;
-    if (!de || (count > 0 && (!dy || !tokens || !workspace))) { set_error("embedding_grad: NULL pointer"); return CN_ERR_NULL; }
-    if (workspace_bytes < cn_embedding_grad_workspace_bytes(count, rows, cols)) {
-        set_error("embedding_grad: workspace of %zu bytes, %zu needed", workspace_bytes, cn_embedding_grad_workspace_bytes(count, rows, cols));
+    const size_t needed = cn_embedding_grad_workspace_bytes(count, rows, cols);
+    if (!de || (count > 0 && (!dy || !tokens)) || (needed > 0 && !workspace)) { set_error("embedding_grad: NULL pointer"); return CN_ERR_NULL; }
+    if (workspace_bytes < needed) {
+        set_error("embedding_grad: workspace of %zu bytes, %zu needed", workspace_bytes, needed);
         return CN_ERR_WORKSPACE;
     }
-    if (count > 0 && !aligned_to(workspace, 256)) { set_error("embedding_grad: the workspace is not aligned to 256 bytes"); return CN_ERR_ARG; }
+    if (needed > 0 && !aligned_to(workspace, 256)) { set_error("embedding_grad: the workspace is not aligned to 256 bytes"); return CN_ERR_ARG; }
     if (count > 0 && de == dy) { set_error("embedding_grad: the gradient is the errors"); return CN_ERR_ARG; }
     const GradPlan p = plan_grad(count, rows, cols);
     const int64_t most = (p.chunks < kDirectItems ? kDirectItems : p.chunks) + (accumulate ? 0 : rows / kZeroRows + 1);
@@ -736,7 +741,7 @@ cn_status cn_embedding_grad(const void *dy, int dy_dtype, int64_t ldy, const voi
     const int64_t vec = 16 / (int64_t)dtype_bytes(dy_dtype);
     const bool wide = cols % vec == 0 && ldy % vec == 0 && lde % vec == 0 && aligned_to(dy, 16) &&
                       aligned_to(de, (size_t)vec * dtype_bytes(de_dtype));
-    const bool direct = count > 0 && count <= kDirectItems && cols <= kDirectSlabs * kDirectLanes * (wide ? vec : 1);
+    const bool direct = never_sorted(count, cols) || (count > 0 && count <= kDirectItems && cols <= kDirectSlabs * kDirectLanes * (wide ? vec : 1));
     int sorted = 0;
     if (count > 0 && !direct) {
         s = token_bits == 32 ? sort_tokens((const int32_t *)tokens, count, rows, p, space, &sorted, st)

@@ -368,8 +368,8 @@ cn_status cn_embedding(const void *table_device, int dtype, int64_t rows, int64_
  * accumulate != 0: the sums are added to dE, and rows that no token names are left as they are: with scale = -rate it is
  * the update of the reference's kUpdateVocabWithGradient.
  * dY: count x cols of dy_dtype; dE: rows x cols, fp32 or of dy_dtype (then added up in fp32 and rounded once).
- * `workspace`: cn_embedding_grad_workspace_bytes(count, rows, cols) bytes of device memory, aligned to 256, the caller's
- * until the call has run; calls with workspaces of their own may overlap.  dE must not overlap dY. */
+ * `workspace`: cn_embedding_grad_workspace_bytes(count, rows, cols) bytes of device memory (0 for few tokens and narrow rows:
+ * then it may be NULL), aligned to 256, the caller's until the call has run; calls with workspaces of their own may overlap.  dE must not overlap dY. */
 size_t cn_embedding_grad_workspace_bytes(int64_t count, int64_t rows, int64_t cols);
 cn_status cn_embedding_grad(const void *dY_device, int dy_dtype, int64_t ldy, const void *tokens_device,
                             int token_bits, int64_t count, int64_t rows, int64_t cols, float scale, int accumulate,

@@ -36,9 +36,9 @@ def test_embedding_refuses():
 def test_embedding_grad_refuses():
     L = cn.lib()
     f, need = L.cn_embedding_grad, L.cn_embedding_grad_workspace_bytes
-    size = need(100, 50, 8)
-    assert size > 100 * 16 and need(0, 50, 8) == 0 and need(100, 50, 0) == 0 and need(-1, 50, 8) == 0
-    ok = [AT, 0, 8, AT, 32, 100, 50, 8, 1.0, 0, AT, 0, 8, AT, size, None]
+    size = need(3000, 50, 8)
+    assert size > 3000 * 16 and need(0, 50, 8) == 0 and need(3000, 50, 0) == 0 and need(-1, 50, 8) == 0 and need(100, 50, 8) == 0
+    ok = [AT, 0, 8, AT, 32, 3000, 50, 8, 1.0, 0, AT, 0, 8, AT, size, None]
 
     def call(**change):
         a = list(ok)
@@ -61,7 +61,7 @@ def test_embedding_grad_refuses():
     _refused(call(_13=AT + 16), ARG)          # alignment of the workspace
     assert call(_5=0, _9=1, _0=None, _3=None, _13=None, _14=0) == 0
     _refused(call(), ARG)                     # onto the errors
-    big = need(100, 2 ** 30, 8)
+    big = need(3000, 2 ** 30, 8)
     _refused(call(_10=2 * AT, _6=2 ** 30, _14=big), SHAPE)             # 2^25 workgroups that write zeros
     _refused(call(_10=2 * AT, _9=1, _7=2 ** 22 + 64, _2=2 ** 23, _12=2 ** 23, _14=2 ** 62), SHAPE)
 
