@@ -583,7 +583,8 @@ def _tokens(tokens, device):
 
 def embedding(table, tokens, scale=1.0, out=None):
     """scale * table[tokens], of shape tokens.shape + (cols,) and the table's type: one row of the table (rows x cols,
-    float32, float16 or bfloat16) per token (int32 or int64), zeros for a token outside the table (padding)."""
+    float32, float16 or bfloat16) per token (int32 or int64), zeros for a token outside the table (padding).  `out` is a
+    matrix of a row per token."""
     import torch
     code = _dtype_code(table, "table")
     bits = _tokens(tokens, table.device)
@@ -610,7 +611,10 @@ def embedding_grad(dY, tokens, rows, scale=1.0, out=None, out_dtype=None, accumu
     `out` and rows that no token names are not touched: scale = -rate makes it the update of the table itself."""
     import torch
     if isinstance(dY, torch.Tensor) and dY.dim() != 2 and dY.dim() > 0:
-        dY = dY.view(-1, dY.shape[-1])
+        try:
+            dY = dY.view(dY.shape[:-1].numel(), dY.shape[-1])
+        except RuntimeError:
+            raise ValueError("dY must be rows in order, with one stride between them")
     code = _dtype_code(dY, "dY")
     bits = _tokens(tokens, dY.device)
     count, cols = dY.shape

@@ -201,6 +201,12 @@ def test_gradient_of_nothing(torch):
     assert not out.any()
     assert cn.embedding_grad(torch.empty(5, 0, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda"), 3).shape == (3, 0)
     assert cn.embedding_grad(torch.ones(5, 4, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda"), 0).shape == (0, 4)
+    windows = torch.zeros(5, 3, dtype=torch.int32, device="cuda")
+    assert cn.embedding_grad(torch.empty(5, 3, 0, device="cuda"), windows, 7).shape == (7, 0)
+    assert not cn.embedding_grad(torch.empty(0, 3, 4, device="cuda"), windows[:0], 7).any()
+    assert torch.equal(cn.embedding_grad(torch.ones(4, device="cuda"), windows[0, 0], 2), torch.tensor([[1.0] * 4, [0.0] * 4], device="cuda"))
+    with pytest.raises(ValueError):  # rows of a window lie apart in another way than windows do
+        cn.embedding_grad(torch.ones(5, 4, 3, device="cuda")[:, :3], windows, 7)
 
 
 def test_a_row_that_is_not_finite_stays_its_own(torch):
