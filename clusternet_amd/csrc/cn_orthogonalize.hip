@@ -11,8 +11,8 @@
 // above the diagonal are computed).  In fp32 the matrix cores give 157 TFLOP/s; here each operand is kept as two fp16
 // numbers, x 2^14 = hi + lo (2^10 for P and Q), and a product is the three fp16 products hi hi + hi lo + lo hi in fp32
 // accumulators.  What is left out, lo lo, and the rounding of lo are 2^-22 of the product, so the result is about as far from
-// the exact one as plain fp32 products leave it (0.55 to 1.35 times as far at twelve sizes from 3000 x 16 to 16384 x 2048, up to
-// 1.8 times at tens of rows, where nothing averages out).  The factors keep entries below 65504 (|X| <= 1.21, |A|, |T| <= 1.46,
+// the exact one as plain fp32 products leave it (0.5 to 1.35 times as far at sixteen sizes from 17 x 498 to 16384 x 2048 of Gaussian
+// numbers, up to 1.8 times at tens of rows, where nothing averages out, and with dominating directions).  The factors keep entries below 65504 (|X| <= 1.21, |A|, |T| <= 1.46,
 // |P| <= 2.81, |Q| <= 41) and lo above the smallest fp16 number for entries down to 2^-13 of the largest.  a X stays outside
 // the product, with X read back as hi + lo: folding a into P's diagonal costs a factor of three in accuracy for nearly
 // low-rank gradients.
@@ -740,13 +740,23 @@ __global__ __launch_bounds__(256) void join_kernel(Product g, int from) {
     f32x16 sum;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
-    for (int part = 0; part < a.parts; ++part) {
-        const float *p = g.parts + (size_t)(a.slot + part * a.count + tile - a.first) * TILE * TILE + block * 1024 + lane * 4;
+    constexpr int kBatch = 4;  // parts in flight: few tiles of a long k have dozens each
+    for (int first = 0; first < a.parts; first += kBatch) {
+        f32x4 x[kBatch][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(p + q * 256);
+        for (int j = 0; j < kBatch; ++j) {
+            if (first + j >= a.parts) break;
+            const float *p = g.parts + (size_t)(a.slot + (first + j) * a.count + tile - a.first) * TILE * TILE + block * 1024 + lane * 4;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[4 * q + e] += x[e];
+            for (int q = 0; q < 4; ++q) x[j][q] = *reinterpret_cast<const f32x4 *>(p + q * 256);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (first + j >= a.parts) break;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[4 * q + e] += x[j][q][e];
         }
     }
     finish_block<FINISH>(g, *g.factor, sum, old, i0, j0, !(g.triangle && ti == tj), stage[wave]);
@@ -761,7 +771,8 @@ struct Cut {
     int whole;  // tiles before the first group with parts
 };
 constexpr int kSlots = 256;  // workgroups at a time, one per compute unit
-Cut cut_with(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, int terms, int tile, bool whole) {
+// At most `most_parts` parts to a tile; 1: whole tiles.
+Cut cut_with(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, int terms, int tile, int most_parts) {
     Cut c{};
     const int64_t ti = (rows_i + tile - 1) / tile, tj = (rows_j + tile - 1) / tile;
     c.tile = tile;
@@ -780,11 +791,13 @@ Cut cut_with(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, int t
         add(kSlots, 1, left / kSlots);
         left %= kSlots;
     }
-    if (whole) {
+    if (most_parts == 1) {
         if (left) add(left, 1, 1);
         return c;
     }
-    const int least = tile == 256 ? 8 : 4, most = c.stages / least < 1 ? 1 : c.stages / least;  // a part has `least` stages or more
+    const int least = tile == 256 ? 8 : 4;  // a part has so many stages or more
+    int most = c.stages / least < 1 ? 1 : c.stages / least;
+    if (most > most_parts) most = most_parts;
     while (left > 0) {
         const bool final = c.groups + 1 == kMaxGroups;
         int parts = final ? kSlots / left : (kSlots + left - 1) / left;
@@ -797,30 +810,32 @@ Cut cut_with(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, int t
     return c;
 }
 // The time a cut is expected to take, in microseconds: what its workgroups do one after the other, and the join.  Measured on
-// 784 x 1024, 1000 x 4001, 4096 x 4096 and 4096 x 16384: a stage's time by tile size and parts per operand, a tile's
-// epilogue, storing a part; a launch takes 4 us more than what runs in it, the parts are written and read at about 8 TB/s together.
+// 784 x 1024, 1000 x 4001, 4096 x 4096 and 4096 x 16384: a stage's time by tile size and number of products, a tile's
+// epilogue, storing a part; a launch takes 4 us more than what runs in it, the parts are written and read at about 8 TB/s together,
+// and the parts of a tile take 0.25 us each one after the other (64 x 16384 in 64 parts: 185 us, in 16 127).
 double cost_of(const Cut &c, int terms) {
     const int size = c.tile == 256 ? 0 : c.tile == 128 ? 1 : 2;
-    static const double stage[3][3] = {{2.1, 1.75, 2.42}, {1.2, 1.2, 1.55}, {0.55, 0.5, 0.53}};  // [size][products - 1]
+    static const double stage[3][3] = {{2.1, 2.07, 2.42}, {1.2, 1.28, 1.55}, {0.55, 0.52, 0.53}};  // [size][products - 1]
     static const double finish[3] = {13.0, 3.0, 1.5}, store[3] = {3.0, 2.0, 1.0};
     double t = 4.0;
-    int busy = 0;
+    int busy = 0, parts = 0;
     for (const Group &g : c.group) {
         if (g.count == 0) continue;
         // a chip that is not full runs at a higher clock
         const double one = stage[size][terms - 1] * (size < 2 && g.count * g.parts < 200 ? 0.72 : 1.0);
         t += g.rounds * (c.stages / (double)g.parts * one + (g.parts > 1 ? store[size] : finish[size]));
         busy += g.parts > 1 ? g.count * g.parts : 0;
+        if (g.parts > parts) parts = g.parts;
     }
-    if (busy) t += 4.5 + (double)busy * c.tile * c.tile * 8 / 8e6;
+    if (busy) t += 4.5 + 0.25 * parts + (double)busy * c.tile * c.tile * 8 / 8e6;
     return t;
 }
 Cut cut_product(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, int terms) {
     Cut best{};
     double least = 0.0;
     for (int tile : {256, 128, 64})
-        for (bool whole : {true, false}) {
-            const Cut c = cut_with(rows_i, rows_j, depth, triangle, terms, tile, whole);
+        for (int most_parts : {1, 16, kSlots}) {
+            const Cut c = cut_with(rows_i, rows_j, depth, triangle, terms, tile, most_parts);
             const double t = cost_of(c, terms);
             if (best.tile == 0 || t < least) {
                 best = c;
