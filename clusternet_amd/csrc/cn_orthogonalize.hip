@@ -856,6 +856,7 @@ struct Sizes {
     int flip, grouped;
     Cut gram[2], square, apply[2];  // [all parts of X, or of an exact X0 hi alone]
 };
+constexpr int64_t kFewRows = 128;
 Sizes sizes_of(int64_t rows, int64_t cols) {
     Sizes z;
     z.flip = rows > cols;
@@ -870,7 +871,9 @@ Sizes sizes_of(int64_t rows, int64_t cols) {
     }
     // Steps in groups, by the products of five steps: 2 of each size n and 14 small ones against 5 and 5.
     const double large = cost_of(z.gram[0], 3) + cost_of(z.apply[0], 3), small = cost_of(z.square, 3);
-    z.grouped = 2 * large + 14 * small < 5 * (large + small);
+    // Not for few rows: all their singular values may be large, then Q is nearly -a^3 on the diagonal, and its rounding counts beside
+    // (a^3 + Q) X with little to average it out (16 x 3000: 2.5 10^-6 of |out|, 1.1 10^-6 by single steps and in plain fp32).
+    z.grouped = z.m > kFewRows && 2 * large + 14 * small < 5 * (large + small);
     return z;
 }
 

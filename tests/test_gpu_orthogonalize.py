@@ -136,6 +136,25 @@ def test_against_plain_32_bits(torch):
             assert ours <= max(1e-6, 1.5 * plain), (rows, cols, kind, ours, plain)
 
 
+@pytest.mark.parametrize("rows,cols", [(3000, 16), (17, 500), (60, 3000), (120, 2500), (140, 5000), (1000, 4001)])
+@pytest.mark.parametrize("kind", ["noise", "strong"])
+def test_long_matrices_against_plain_32_bits(torch, rows, cols, kind):
+    """Operands in two parts are rounded to 2^-23, twice fp32's 2^-24: at most twice as far, and 1e-6 for what is left to chance
+    where both are that near."""
+    import clusternet_amd as cn
+    G = _gradient(torch, rows, cols, 31, kind)
+    want = _exact(torch, G)
+    x = (G if rows <= cols else G.T).contiguous()
+    x = x / (x.norm() + 1e-7)
+    for _ in range(5):
+        a = x @ x.T.contiguous()
+        x = A * x + (B * a + C * (a @ a)) @ x
+    x = x if rows <= cols else x.T
+    plain = float((x.double() - want).norm() / want.norm())
+    ours = float((cn.orthogonalize(G).double() - want).norm() / want.norm())
+    assert ours <= max(1e-6, 2 * plain), (ours, plain)
+
+
 def test_scale_does_not_matter(torch):
     """Gradients of any finite size: powers of two change nothing until 1e-7 counts, and sums of squares do not overflow."""
     import clusternet_amd as cn
