@@ -24,7 +24,8 @@
 // or three behind two, errors grow tenfold (emulated in 64 bits on Gaussian, orthogonal, rank-one, nearly low-rank spectra and
 // power laws), with three and two they stay at those of plain fp32.  Measured, steps alone -> in groups: 4096 x 16384 bf16
 // 10.8 -> 6.65 ms, 1000 x 4001 384 -> 319 us, 1000 x 2000 283 -> 272, but 784 x 1024 186 -> 215 and 4096 x 4096 3.91 -> 4.27 ms:
-// taken where the products' estimated times add up to less (sizes_of; at twelve sizes at most 3 % off the better form).
+// taken for more than 128 rows where the products' estimated times add up to less (sizes_of; at twelve sizes at most 3 %
+// off the better form).
 //
 // A gradient of 16 bits is its own hi if only the power of two of the scale is applied to it, so X0 X0^T is one product and Q X0
 // two, with nothing lost; the rest of the scale, in [1, 2), goes to their results (split_kernel).  (One product in place of
