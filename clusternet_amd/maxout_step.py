@@ -40,23 +40,33 @@ def sparse_input(X):
 
 
 class TokenInput:
-    """Windows of words: the table (rows x D), the tokens (batch x window) and X (batch x window * D), their rows."""
+    """Windows of words: the table (rows x D) and the tokens (batch x window).  It holds no rows: the table moves with every step."""
 
-    def __init__(self, table, tokens, scale, X):
-        self.table, self.tokens, self.scale, self.X = table, tokens, scale, X
+    def __init__(self, table, tokens, scale=1.0):
+        if tokens.dim() != 2:
+            raise ValueError("tokens must be batch x window")
+        L._dtype_code(table, "table")
+        L._tokens(tokens, table.device)
+        self.table, self.tokens, self.scale = table, tokens, scale
+
+    @property
+    def X(self):
+        """The rows of the words as the table holds them now, batch x window * D: a lookup each time."""
+        X = L.embedding(self.table, self.tokens, self.scale)
+        return X.view(X.shape[0], X.shape[1] * X.shape[2])
 
 
 def token_input(table, tokens, scale=1.0):
-    if tokens.dim() != 2:
-        raise ValueError("tokens must be batch x window")
-    X = L.embedding(table, tokens, scale)
-    return TokenInput(table, tokens, scale, X.view(X.shape[0], X.shape[1] * X.shape[2]))
+    return TokenInput(table, tokens, scale)
 
 
 def forward(X, params, pool=2):
+    """(p, cache).  The cache is h1, a1, h2, a2 and, for a TokenInput, the rows that this forward pass looked up."""
     W1, b1, W2, b2, W3, b3 = params
+    rows = ()
     if isinstance(X, TokenInput):
         X = X.X
+        rows = (X,)
     # bias and maxout are taken in one pass behind each product (inside it for the sparse first layer)
     if isinstance(X, SparseInput):
         h1, a1 = L.csr_gemm_bias_maxout(X.csr, W1, b1, pool)
@@ -64,7 +74,7 @@ def forward(X, params, pool=2):
         h1, a1 = L.dot_bias_maxout(X, W1, b1, pool)
     h2, a2 = L.dot_bias_maxout(h1, W2, b2, pool)
     p = L.softmax(L.add_row_vector(L.dot(h2, W3), b3))
-    return p, (h1, a1, h2, a2)
+    return p, (h1, a1, h2, a2) + rows
 
 
 def backward(X, onehot, params, p, cache, pool=2, absmax_out=None, defer_first=False):
@@ -76,7 +86,7 @@ def backward(X, onehot, params, p, cache, pool=2, absmax_out=None, defer_first=F
     W1, b1, W2, b2, W3, b3 = params
     words = isinstance(X, TokenInput)
     if words:
-        X = X.X
+        X, cache = cache[4], cache[:4]
     h1, a1, h2, a2 = cache
     m1, m2, m3 = absmax_out if absmax_out is not None else (None, None, None)
     e3 = L.sub(p, onehot)
