@@ -156,7 +156,10 @@ def coded_rmsprop_update(w, rms, grad, rms_multiplier, rate, fused=True, scratch
 
 
 def step(X, onehot, params, rate, pool=2):
+    """One step by 8-bit gradients on a dense batch or a SparseInput.  For a TokenInput, whose table moves too: `token_step`."""
     import torch
+    if isinstance(X, TokenInput):
+        raise TypeError("step has no rate for the table of a TokenInput: use token_step")
     p, cache = forward(X, params, pool)
     maxima = [torch.empty(1, dtype=torch.float32, device=p.device) for _ in range(3)]
     sparse = isinstance(X, SparseInput)
