@@ -184,11 +184,12 @@ def token_step(X, onehot, params, momenta, rate, table_rate, momentum_factor=0.9
     """One step on a TokenInput: W1 and W2 along the orthogonalised `momenta` (two matrices of their shapes), W3 by its 8-bit
     gradient, and the table."""
     import torch
+    mom1, mom2 = momenta
     p, cache = forward(X, params, pool)
     m3 = torch.empty(1, dtype=torch.float32, device=p.device)
     gW1, gW2, gW3, e0 = backward(X, onehot, params, p, cache, pool, absmax_out=(None, None, m3))
-    for w, m, g in zip((params[0], params[2]), momenta, (gW1, gW2)):
-        L.muon_update(m, g, w, momentum_factor, rate)
+    L.muon_update(mom1, gW1, params[0], momentum_factor, rate)
+    L.muon_update(mom2, gW2, params[2], momentum_factor, rate)
     coded_update(params[4], gW3, coded_rate, prec=m3)
     table_update(X, e0, table_rate)
     return p
