@@ -197,7 +197,7 @@ def token_step(X, onehot, params, momenta, rate, table_rate, momentum_factor=0.9
 
 def quantize_params(params, group=128, zero_points=False):
     """The parameters with their three matrices in 4 bits, for `answer`."""
-    return tuple(L.quantize_4bit(t, group, zero_points) if t.dim() == 2 else t for t in params)
+    return tuple(t if bias else L.quantize_4bit(t, group, zero_points) for t, bias in zip(params, (0, 1, 0, 1, 0, 1)))
 
 
 def answer(X, params4, pool=2):

@@ -80,3 +80,14 @@ def test_one_captured_input(torch):
         assert torch.equal(p, p2)
         for a, b in zip([table, *params, *momenta], [table2, *params2, *momenta2]):
             assert torch.equal(a, b)
+
+
+def test_answers_with_biases_of_any_shape(torch):
+    from clusternet_amd import maxout_step as ms
+    table, params, _, tokens, _ = _net(torch, 5)
+    X = ms.token_input(table, tokens)
+    want = ms.answer(X, ms.quantize_params(params))
+    for shape in ((1, -1), (-1, 1)):
+        shaped = [t if i % 2 == 0 else t.view(shape) for i, t in enumerate(params)]
+        assert torch.equal(ms.forward(X, shaped)[0], ms.forward(X, params)[0])
+        assert torch.equal(ms.answer(X, ms.quantize_params(shaped)), want)
