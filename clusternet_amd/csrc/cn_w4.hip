@@ -13,6 +13,10 @@
 //     give exactly 16 + q, a shift and an and-or for two weights.  The 16 and the zero point leave again behind the sum:
 //         sum a (q - z) = sum a (16 + q) - (16 + z) sum a,
 //     where sum a comes from one more matrix instruction against ones, in the same fp32 accumulators and the same order.
+//     Where a may be as large as fp32 goes, both sums are of 2^-13 (16 + q) and 2^-13 in place of 16 + q and 1 (another
+//     exponent in the same pattern): 128 * 31 of them stay below 2^128, where they were infinite, and their difference NaN, from
+//     |a| = 8 10^34 on.  The 2^13 comes back in the write-out: all sums keep 2^-136, half a step of the smallest normal bf16
+//     number.  (Given to the scales, which then need a place for those above 2^115: 5 % for groups of 32.)
 //   * Products are exact: a 16-bit a times a whole number up to 31 fits fp32; a of fp32 enters as three bf16 numbers that add
 //     up to it exactly (8 bits of it each).  The sums, the scales and everything behind them are fp32; a 16-bit result is
 //     rounded once.
@@ -53,7 +57,8 @@ struct GemmW4Args {
 template <typename T> struct Kind;
 template <> struct Kind<bf16_t> {
     static constexpr int kParts = 1;
-    static constexpr uint32_t kMagic = 0x41804180u, kMask = 0x00780078u, kOnes = 0x3f803f80u;
+    static constexpr uint32_t kMagic = 0x3b003b00u, kMask = 0x00780078u, kOnes = 0x39003900u;  // 2^-9 = 16 / kUnit, 1 / kUnit
+    static constexpr float kUnit = 8192.0f;
     static constexpr int kShift = 3;
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -65,6 +70,7 @@ template <> struct Kind<float> : Kind<bf16_t> {
 template <> struct Kind<f16_t> {
     static constexpr int kParts = 1;
     static constexpr uint32_t kMagic = 0x4c004c00u, kMask = 0x03c003c0u, kOnes = 0x3c003c00u;
+    static constexpr float kUnit = 1.0f;  // 128 * 31 of the largest fp16 number fit fp32
     static constexpr int kShift = 6;
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -302,7 +308,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
         float v = sums[at];
 #pragma unroll
         for (int wv = 1; wv < WAVES; ++wv) v += sums[wv * MB * NT * 256 + at];
-        ((T *)g.out)[(m0 + m) * g.ldo + n0 + n] = (T)v;
+        ((T *)g.out)[(m0 + m) * g.ldo + n0 + n] = (T)(v * Q::kUnit);
     }
 }
 
