@@ -9,14 +9,21 @@
 // padded with code 0 to whole tiles.
 //
 // Product: out[M x N] = A W, bound by the codes' way from memory for up to a few dozen rows.
-//   * Codes become numbers without arithmetic: bits 3 .. 6 of the bf16 pattern of 16.0 (bits 6 .. 9 of the fp16 one) set to q
-//     give exactly 16 + q, a shift and an and-or for two weights.  The 16 and the zero point leave again behind the sum:
+//   * 16-bit rows: codes become numbers without arithmetic.  Bits 3 .. 6 of the bf16 pattern of 16.0 (bits 6 .. 9 of the fp16 one)
+//     set to q give exactly 16 + q, a shift and an and-or for two weights.  The 16 and the zero point leave again behind the sum:
 //         sum a (q - z) = sum a (16 + q) - (16 + z) sum a,
-//     where sum a comes from one more matrix instruction against ones, in the same fp32 accumulators and the same order.
-//     Where a may be as large as fp32 goes, both sums are of 2^-13 (16 + q) and 2^-13 in place of 16 + q and 1 (another
-//     exponent in the same pattern): 128 * 31 of them stay below 2^128, where they were infinite, and their difference NaN, from
-//     |a| = 8 10^34 on.  The 2^13 comes back in the write-out: all sums keep 2^-136, half a step of the smallest normal bf16
-//     number.  (Given to the scales, which then need a place for those above 2^115: 5 % for groups of 32.)
+//     where sum a comes from one more matrix instruction against ones, in the same fp32 accumulators and the same order.  For rows
+//     with a mean the difference is far smaller than its two sums, and their roundings with it (5 10^-6 of the largest result
+//     for maxout outputs, 1 x 4096): little beside a 16-bit result's rounding (21 of 16384 bf16 results are not the exact ones rounded,
+//     8 in plain fp32), too much for fp32.
+//   * So fp32 rows take q - z, exact in bf16 and 15 operations more for eight weights, which cost what the product with ones did
+//     (13 x 5000 x 1999 13.4 us, with 16 + q 13.1; 64 x 8192 x 16384 91 and 86, 40 x 8192 x 8192 in groups of 32 67 and 72).
+//     The errors are 0.16 to 0.31 of those of a plain fp32 product of the decoded weights (root mean square, rows of mean zero,
+//     maxout and sigmoid outputs, rows near 1), where they were up to 35 times those.
+//   * Where a may be as large as fp32 goes, the operands are 2^-13 (16 + q), 2^-13 in place of 1, and 2^-11 (q - z) (another
+//     exponent in the same pattern): 128 of the largest fit fp32, where same-signed rows from 8 10^34 on would overflow.
+//     The factor comes back in the write-out: all sums keep 2^-136, half a step of the smallest normal bf16 number.  (Given
+//     to the scales, which then need a place for those above 2^115: 5 % for groups of 32.)
 //   * Products are exact: a 16-bit a times a whole number up to 31 fits fp32; a of fp32 enters as three bf16 numbers that add
 //     up to it exactly (8 bits of it each).  The sums, the scales and everything behind them are fp32; a 16-bit result is
 //     rounded once.
@@ -66,7 +73,9 @@ template <> struct Kind<bf16_t> {
 };
 template <> struct Kind<float> : Kind<bf16_t> {
     static constexpr int kParts = 3;
+    static constexpr float kUnit = 2048.0f;
 };
+template <typename T> constexpr bool kCentred = sizeof(T) == 4;  // operands are q - z instead of 16 + q
 template <> struct Kind<f16_t> {
     static constexpr int kParts = 1;
     static constexpr uint32_t kMagic = 0x4c004c00u, kMask = 0x03c003c0u, kOnes = 0x3c003c00u;
@@ -89,6 +98,17 @@ __device__ __forceinline__ u32x4 expand(uint32_t w) {
         const int down = 4 * j - Q::kShift;  // nibble j from bit 4 j to bit kShift
         b[j] = ((down >= 0 ? w >> down : w << -down) & Q::kMask) | Q::kMagic;
     }
+    return b;
+}
+
+// The same of fp32 rows: (q - z) / kUnit, exact in bf16; zero: z / kUnit of the lane's column.  23 operations in place of 8.
+template <typename T>
+__device__ __forceinline__ u32x4 expand_centred(uint32_t w, float zero) {
+    const uint32_t nibbles[2] = {w & 0x0f0f0f0fu, w >> 4 & 0x0f0f0f0fu};  // byte m: nibble 2 m, 2 m + 1
+    auto weight = [&](int i) { return __builtin_fmaf((float)(nibbles[i & 1] >> (8 * (i >> 1)) & 255u), 1.0f / Kind<T>::kUnit, -zero); };
+    u32x4 b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = __builtin_amdgcn_perm(__float_as_uint(weight(j + 4)), __float_as_uint(weight(j)), 0x07060302u);
     return b;
 }
 
@@ -222,19 +242,29 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
     auto consume = [&](const Slot &s, const u32x4 (&a)[kAheadA ? 4 : 1][kRaw], int kb, int next, auto whole) {
         constexpr bool kWhole = decltype(whole)::value != 0;
         f32x4 acc[MB][NT], sum_a[MB];
+        float zero[NT];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+            auto of_group = [&](float v) {
+                return GROUPS == 1 ? v : __uint_as_float(__builtin_amdgcn_ds_bpermute((q / kSpan * 16 + c) * 4, (int)__float_as_uint(v)));
+            };
             if (q % kSpan == 0) {
 #pragma unroll
                 for (int b = 0; b < MB; ++b) {
-                    sum_a[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (!kCentred<T>) sum_a[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int t = 0; t < NT; ++t) acc[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
                 }
+                if (kCentred<T>)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) zero[t] = of_group(s.zero[t]) * (1.0f / Q::kUnit);
             }
             u32x4 bw[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) bw[t] = expand<T>(s.w[t][q]);
+            for (int t = 0; t < NT; ++t) {
+                if constexpr (kCentred<T>) bw[t] = expand_centred<T>(s.w[t][q], zero[t]);
+                else bw[t] = expand<T>(s.w[t][q]);
+            }
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
                 u32x4 raw[kRaw], part[kParts];
@@ -247,7 +277,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
                 operand<T>(raw, part);
 #pragma unroll
                 for (int p = kParts - 1; p >= 0; --p) {
-                    sum_a[b] = Q::mfma(part[p], ones, sum_a[b]);
+                    if (!kCentred<T>) sum_a[b] = Q::mfma(part[p], ones, sum_a[b]);
 #pragma unroll
                     for (int t = 0; t < NT; ++t) acc[b][t] = Q::mfma(part[p], bw[t], acc[b][t]);
                 }
@@ -256,15 +286,14 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_w4_kernel(GemmW4Args g) {
             if (q % kSpan == kSpan - 1) {  // the end of a group
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    auto of_group = [&](float v) {
-                        return GROUPS == 1 ? v : __uint_as_float(__builtin_amdgcn_ds_bpermute((q / kSpan * 16 + c) * 4, (int)__float_as_uint(v)));
-                    };
-                    const float scale = of_group(s.scale[t]), offset = 16.0f + of_group(s.zero[t]);
+                    const float scale = of_group(s.scale[t]), offset = kCentred<T> ? 0.0f : 16.0f + of_group(s.zero[t]);
 #pragma unroll
                     for (int b = 0; b < MB; ++b)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            total[b][t][r] = __builtin_fmaf(scale, __builtin_fmaf(-offset, sum_a[b][r], acc[b][t][r]), total[b][t][r]);
+                        for (int r = 0; r < 4; ++r) {
+                            const float sum = kCentred<T> ? acc[b][t][r] : __builtin_fmaf(-offset, sum_a[b][r], acc[b][t][r]);
+                            total[b][t][r] = __builtin_fmaf(scale, sum, total[b][t][r]);
+                        }
                 }
             }
         }

@@ -315,9 +315,12 @@ cn_status cn_dequantize_4bit(const int32_t *codes_device, const float *scales_de
                              int64_t K, int64_t N, int group, void *out_device, int dtype, int64_t ldo, void *stream);
 
 /* out (M x N) = A (M x K) W with W in that form; A and out of `dtype`.  Products are exact, sums and scales fp32, a
- * 16-bit result is rounded once.  Made for answers (a row per token, up to a few dozen); any M is right, but from a few
- * hundred rows on decoded weights are faster.  The same bits every time; needs no workspace.  out must not overlap A.  A row of A with a number
- * that is not finite gives NaNs.  The 8-bit relative is cn_gemm_f32_w8. */
+ * 16-bit result is rounded once.  For fp32 the result is at least as near as a plain fp32 product of the decoded weights;
+ * for 16 bits the sums carry 16 + q in place of q - z, so that their fp32 roundings are up to some 10 times those of such a
+ * product, 10^-5 of the largest result.  Any finite A whose sums of |a w| are finite; what is below 2^-136 may be lost.  Made for
+ * answers (a row per token, up to a few dozen); any M is right, but from a few hundred rows on decoded weights are
+ * faster.  The same bits every time; needs no workspace.  out must not overlap A.  A row of A with a number that is not
+ * finite gives NaNs.  The 8-bit relative is cn_gemm_f32_w8. */
 cn_status cn_gemm_w4(int64_t M, int64_t N, int64_t K, const void *A_device, int dtype, int64_t lda,
                      const int32_t *codes_device, const float *scales_device, const uint8_t *zeros_device, int group,
                      void *out_device, int64_t ldo, void *stream);
