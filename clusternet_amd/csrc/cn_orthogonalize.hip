@@ -69,13 +69,17 @@ int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
 __device__ __forceinline__ size_t split_at(int64_t row, int64_t col, int64_t cols) {
     return ((size_t)(row >> 8) * (size_t)(cols >> 5) + (size_t)(col >> 5)) * (256 * 64) + (size_t)(row & 255) * 64 + (col & 31);
 }
-// Four consecutive columns (col a multiple of 4), in stored units.
+// Four consecutive columns (col a multiple of 4), in stored units.  What a number was computed with is hidden from its
+// conversion: a product that becomes fp16 by one fused instruction in the one place and is rounded to fp32 before in the other gave
+// two different hi where it was near a tie (one of 10^4 elements of A for 16-bit gradients, each off by 2^-11 of itself).
 __device__ __forceinline__ void split_store(f16_t *m, size_t at, const float (&v)[4]) {
     f16x4 hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        hi[e] = (f16_t)v[e];
-        lo[e] = (f16_t)(v[e] - (float)hi[e]);
+        float x = v[e];
+        asm("" : "+v"(x));
+        hi[e] = (f16_t)x;
+        lo[e] = (f16_t)(x - (float)hi[e]);
     }
     *reinterpret_cast<f16x4 *>(m + at) = hi;
     *reinterpret_cast<f16x4 *>(m + at + 32) = lo;
