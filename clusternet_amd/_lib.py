@@ -638,7 +638,7 @@ def embedding_grad(dY, tokens, rows, scale=1.0, out=None, out_dtype=None, accumu
 
 
 def orthogonalize(G, steps=5, out=None):
-    """G with its singular values moved towards one by `steps` Newton-Schulz steps, to the accuracy of fp32 products,
+    """G with its singular values moved towards one by `steps` Newton-Schulz steps, about as near as fp32 products,
     rounded once; `out` (G's type if not given; float32, float16 or bfloat16) may be G itself."""
     import torch
     code = _dtype_code(G, "G")

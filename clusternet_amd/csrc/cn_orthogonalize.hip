@@ -9,25 +9,21 @@
 //
 // The products are what this costs: 3 m^2 n + m^3 multiply-adds per step after the symmetry of A and A A (only tiles on and
 // above the diagonal are computed).  In fp32 the matrix cores give 157 TFLOP/s; here each operand is kept as two fp16
-// numbers, x 2^14 = hi + lo (2^10 for P and Q), and a product is the three fp16 products hi hi + hi lo + lo hi in fp32
+// numbers, x 2^14 = hi + lo (2^10 for P), and a product is the three fp16 products hi hi + hi lo + lo hi in fp32
 // accumulators.  What is left out, lo lo, and the rounding of lo are 2^-22 of the product, so the result is about as far from
-// the exact one as plain fp32 products leave it (0.5 to 1.35 times as far at sixteen sizes from 17 x 498 to 16384 x 2048 of Gaussian
-// numbers, up to 1.8 times at tens of rows, where nothing averages out, and with dominating directions).  The factors keep entries below 65504 (|X| <= 1.21, |A|, |T| <= 1.46,
-// |P| <= 2.81, |Q| <= 41) and lo above the smallest fp16 number for entries down to 2^-13 of the largest.  a X stays outside
-// the product, with X read back as hi + lo: folding a into P's diagonal costs a factor of three in accuracy for nearly
-// low-rank gradients.
+// the exact one as plain fp32 products leave it.  Root mean square over gradients, twelve sizes from 16 x 3000 to 4096 x 4096: 0.2 to
+// 1.4 times as far for Gaussian numbers, half of the rows zero, few strong directions; up to 2.4 times (and 1.2 10^-6 of
+// |out|) for gradients of one or two rows or of one column, where roundings do not average out.  The factors keep entries
+// below 65504 (|X| <= 1.21, |A| <= 1.46, |P| <= 2.81) and lo above the smallest fp16 number for entries down to 2^-13 of
+// the largest.  a X stays outside the product, with X read back as hi + lo: folding a into P's diagonal costs a factor of
+// three in accuracy for nearly low-rank gradients.
 //
-// For long matrices several steps are one: A, its polynomials and A' = p A p of the next step (p = a + P) commute, so a group of
-// steps runs on m x m matrices alone, Q = p'' p' p - a^3, and X <- a^3 X + Q X comes once at its end.  A group of g steps costs
-// 3 m^2 n + (4 g - 3) m^3 in place of g (3 m^2 n + m^3), at n = 4 m 42 % less for five steps as three and two.  A is computed from X
-// again after at most three steps in the beginning, where singular values grow, and two later on: with five steps in one group,
-// or three behind two, errors grow tenfold (emulated in 64 bits on Gaussian, orthogonal, rank-one, nearly low-rank spectra and
-// power laws), with three and two they stay at those of plain fp32.  Measured, steps alone -> in groups: 4096 x 16384 bf16
-// 10.8 -> 6.65 ms, 1000 x 4001 384 -> 319 us, 1000 x 2000 283 -> 272, but 784 x 1024 186 -> 215 and 4096 x 4096 3.91 -> 4.27 ms:
-// taken for more than 128 rows where the products' estimated times add up to less (sizes_of; at twelve sizes at most 3 %
-// off the better form).
+// Several steps on m x m matrices alone, with X updated once at their end (A and its polynomials commute; 6.6 ms in place of
+// 10.8 for 4096 x 16384), are not sound in these numbers: the polynomial Q of two or three steps has entries of up to 12 or 41 where a
+// row has a large singular value to itself, and (a^g + Q) X, of about 1, keeps their rounding: 4 10^-6 to 10^-5 of |out| for
+// gradients of one or two rows or of one column, up to twenty times plain fp32.
 //
-// A gradient of 16 bits is its own hi if only the power of two of the scale is applied to it, so X0 X0^T is one product and Q X0
+// A gradient of 16 bits is its own hi if only the power of two of the scale is applied to it, so X0 X0^T is one product and P X0
 // two, with nothing lost; the rest of the scale, in [1, 2), goes to their results (split_kernel).  (One product in place of
 // three in later steps too is not sound: hi alone is off by up to 2^-11 the same way in all equal entries, such as the
 // diagonal of A for orthogonal rows, and the next steps multiply that by ten: 5 10^-3 of |out| for 17 x 498.)
@@ -58,7 +54,7 @@ typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
-constexpr float kUnit = 16384.0f, kPolyUnit = 1024.0f;  // the stored number for 1: of X, A and T, and of P and Q
+constexpr float kUnit = 16384.0f, kPolyUnit = 1024.0f;  // the stored number for 1: of X and A, and of P
 constexpr int kPad = 256;                           // rows and columns are padded to whole tiles
 
 int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
@@ -224,9 +220,8 @@ __global__ __launch_bounds__(256) void split_kernel(Source s, const double *part
 enum Finish {
     GRAM = 0,  // y D, symmetric
     POLY = 1,  // x old + y D, symmetric
-    SUM = 2,   // x old + x2 old2 + y D, symmetric
-    STEP = 3,  // X <- x X + y D^T, both orientations; D = X^T P, n x m
-    LAST = 4   // the same, into the result
+    STEP = 2,  // X <- x X + y D^T, both orientations; D = X^T P, n x m
+    LAST = 3   // the same, into the result
 };
 //
 // Units of work: a group of `count` consecutive tiles, each cut along k into `parts`; workgroup w of a group takes part
@@ -244,9 +239,9 @@ struct Product {
     int triangle;            // the result is symmetric: only tiles with j >= i
     Group group[kMaxGroups];  // unused ones: all 0
     float *parts;            // TILE x TILE numbers per unit of a group with more than one part per tile
-    const f16_t *old, *old2;  // STEP, LAST: X
-    float x, x2, y;           // in stored units
-    const float *factor;      // x and y are multiplied by this
+    const f16_t *old;        // POLY: A; STEP, LAST: X
+    float x, y;              // in stored units
+    const float *factor;     // x and y are multiplied by this
     f16_t *to;                // symmetric results; STEP: X (its own elements only, so in place)
     f16_t *to_t;             // STEP: X^T of the next step (this one's is an operand)
     int64_t to_cols, to_t_cols;
@@ -404,8 +399,6 @@ __device__ __forceinline__ void write_result(const Product &g, int64_t row, int6
 template <int FINISH>
 __device__ __forceinline__ void finish_block(const Product &g, float factor, const f32x16 &sum, const Old &old, int64_t i0, int64_t j0,
                                              bool mirror, float *stage) {
-    Old old2;
-    if (FINISH == SUM) load_old<FINISH>(g, g.old2, i0, j0, old2);
     const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -425,7 +418,6 @@ __device__ __forceinline__ void finish_block(const Product &g, float factor, con
         for (int e = 0; e < 4; ++e) {
             v[e] *= y;
             if (FINISH != GRAM) v[e] = x * ((float)old.hi[p][e] + (float)old.lo[p][e]) + v[e];
-            if (FINISH == SUM) v[e] = g.x2 * ((float)old2.hi[p][e] + (float)old2.lo[p][e]) + v[e];
         }
         const float w[4] = {v[0], v[1], v[2], v[3]};
         if (!last) {
@@ -851,17 +843,16 @@ Cut cut_product(int64_t rows_i, int64_t rows_j, int64_t depth, bool triangle, in
 }
 
 struct Space {
-    f16_t *x, *xt[2], *a, *b[3];
+    f16_t *x, *xt[2], *a, *p;
     float *parts, *factors;
     double *norms;
     size_t bytes;
 };
 struct Sizes {
     int64_t m, n, mp, np;
-    int flip, grouped;
+    int flip;
     Cut gram[2], square, apply[2];  // [all parts of X, or of an exact X0 hi alone]
 };
-constexpr int64_t kFewRows = 128;
 Sizes sizes_of(int64_t rows, int64_t cols) {
     Sizes z;
     z.flip = rows > cols;
@@ -874,11 +865,6 @@ Sizes sizes_of(int64_t rows, int64_t cols) {
         z.gram[exact] = cut_product(z.m, z.m, z.n, true, exact ? 1 : 3);
         z.apply[exact] = cut_product(z.n, z.m, z.m, false, exact ? 2 : 3);
     }
-    // Steps in groups, by the products of five steps: 2 of each size n and 14 small ones against 5 and 5.
-    const double large = cost_of(z.gram[0], 3) + cost_of(z.apply[0], 3), small = cost_of(z.square, 3);
-    // Not for few rows: all their singular values may be large, then Q is nearly -a^3 on the diagonal, and its rounding counts beside
-    // (a^3 + Q) X with little to average it out (16 x 3000: 2.5 10^-6 of |out|, 1.1 10^-6 by single steps and in plain fp32).
-    z.grouped = z.m > kFewRows && 2 * large + 14 * small < 5 * (large + small);
     return z;
 }
 
@@ -889,7 +875,7 @@ Space lay_out(void *workspace, const Sizes &z) {
     s.xt[0] = c.take<f16_t>((size_t)z.mp * z.np * 2);
     s.xt[1] = c.take<f16_t>((size_t)z.mp * z.np * 2);
     s.a = c.take<f16_t>((size_t)z.mp * z.mp * 2);
-    for (int i = 0; i < (z.grouped ? 3 : 1); ++i) s.b[i] = c.take<f16_t>((size_t)z.mp * z.mp * 2);
+    s.p = c.take<f16_t>((size_t)z.mp * z.mp * 2);
     size_t parts = 0;
     for (const Cut *cut : {&z.gram[0], &z.gram[1], &z.square, &z.apply[0], &z.apply[1]}) {
         const size_t need = (size_t)cut->slots * cut->tile * cut->tile;
@@ -928,8 +914,6 @@ struct Result {
     float keep, rate;
 };
 
-constexpr int kFirstGroup = 3, kGroup = 2;  // steps
-
 template <typename T>
 cn_status newton_schulz(const Source &src, int steps, const Result &res, const Sizes &z, const Space &s, int device, hipStream_t st) {
     const int exact = sizeof(T) == 2 && !src.momentum;
@@ -962,64 +946,38 @@ cn_status newton_schulz(const Source &src, int steps, const Result &res, const S
         for (int i = 0; i < kMaxGroups; ++i) g.group[i] = c.group[i];
         return g;
     };
-    // to = x old + y U V of symmetric matrices that commute, in stored units; with old2 SUM.
-    auto square = [&](const f16_t *u, const f16_t *v, const f16_t *old, float x, const f16_t *old2, float x2, float y, f16_t *to) {
-        Product g = with(z.square, u, v, z.mp);
-        g.triangle = 1;
-        g.old = old; g.old2 = old2;
-        g.x = x; g.x2 = x2; g.y = y;
-        g.to = to;
-        g.to_cols = z.mp;
-        return old2 ? run_product<3, SUM>(g, z.square, device, st) : run_product<3, POLY>(g, z.square, device, st);
-    };
-    constexpr float kMixed = kUnit / (kUnit * kPolyUnit);  // y of a product of an operand in each unit whose result is in kUnit
-    int at = 0;                                            // which X^T is current
-    for (int done = 0; done < steps;) {
-        const int most = !z.grouped ? 1 : done == 0 ? kFirstGroup : kGroup, count = steps - done < most ? steps - done : most;
-        const bool hi_alone = exact && done == 0;
+    int at = 0;  // which X^T is current
+    for (int done = 0; done < steps; ++done) {
+        const bool first = done == 0, last = done + 1 == steps, hi_alone = exact && first, two = hi_alone && !last;
         Product g = with(z.gram[hi_alone], s.x, s.x, z.np);
         g.triangle = 1;
         g.y = 1.0f / kUnit;
-        g.factor = s.factors + (done == 0 ? 2 : 0);
+        g.factor = s.factors + (first ? 2 : 0);
         g.to = s.a;
         g.to_cols = z.mp;
         cn_status status = hi_alone ? run_product<1, GRAM>(g, z.gram[1], device, st) : run_product<3, GRAM>(g, z.gram[0], device, st);
-        auto poly = [&](f16_t *to) {
-            return square(s.a, s.a, s.a, kB * kPolyUnit / kUnit, nullptr, 0.0f, kC * kPolyUnit / (kUnit * kUnit), to);
-        };
-        // p: the step's polynomial, q: the group's, t: p A
-        f16_t *p = s.b[0], *q = s.b[0];
-        float q0 = kA;
-        if (status == CN_OK) status = poly(p);
-        for (int k = 1; k < count && status == CN_OK; ++k) {
-            f16_t *t = s.b[0], *next = s.b[0];
-            for (f16_t *b : s.b)
-                if (b != p && b != q) t = b;
-            status = square(s.a, p, s.a, kA, nullptr, 0.0f, kMixed, t);
-            if (status == CN_OK) status = square(p, t, t, kA, nullptr, 0.0f, kMixed, s.a);
-            p = t;
-            if (status == CN_OK) status = poly(p);
-            for (f16_t *b : s.b)
-                if (b != p && b != q) next = b;
-            if (status == CN_OK) status = square(p, q, p, q0, q, kA, 1.0f / kPolyUnit, next);
-            q = next;
-            q0 *= kA;
-        }
         if (status != CN_OK) return status;
-        const bool last = done + count == steps, two = hi_alone && !last;
+        g = with(z.square, s.a, s.a, z.mp);
+        g.triangle = 1;
+        g.old = s.a;
+        g.x = kB * kPolyUnit / kUnit;
+        g.y = kC * kPolyUnit / (kUnit * kUnit);
+        g.to = s.p;
+        g.to_cols = z.mp;
+        status = run_product<3, POLY>(g, z.square, device, st);
+        if (status != CN_OK) return status;
         const Cut &c = z.apply[two];
-        g = with(c, s.xt[at], q, z.mp);
+        g = with(c, s.xt[at], s.p, z.mp);
         g.old = s.x;
-        g.x = q0;
-        g.y = kMixed;
-        g.factor = s.factors + (done == 0 ? 1 : 0);
+        g.x = kA;
+        g.y = 1.0f / kPolyUnit;
+        g.factor = s.factors + (first ? 1 : 0);
         g.to = s.x;
         g.to_cols = z.np;
         g.to_t = s.xt[at ^ 1];
         status = last ? run_product<3, LAST>(g, c, device, st) : two ? run_product<2, STEP>(g, c, device, st) : run_product<3, STEP>(g, c, device, st);
         if (status != CN_OK) return status;
         at ^= 1;
-        done += count;
     }
     return CN_OK;
 }

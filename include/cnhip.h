@@ -333,9 +333,11 @@ cn_status cn_gemm_w4(int64_t M, int64_t N, int64_t K, const void *A_device, int 
 
 /* out = the gradient with its singular values moved towards one: X = G / (|G|_F + 1e-7), transposed if rows > cols, then
  * `steps` times A = X X^T, X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X (five steps bring singular values from 0.002 to 1 of
- * the largest to between about 0.7 and 1.2).  To the accuracy of fp32 products, rounded once; elements of X0 below 2^-38 count as
- * zero (so does a gradient whose norm is that far below 1e-7).  G and out are rows x cols, CN_F32, CN_F16 or CN_BF16 each; out
- * may be G.  A zero G gives zeros, one that is not finite NaNs. */
+ * the largest to between about 0.7 and 1.2).  Operands have 22 to 23 bits (two fp16 numbers), sums are fp32: about as far
+ * from the exact result as plain fp32 products, 0.2 to 1.4 times for most gradients, at most three times (root mean square)
+ * where one row or column is all there is; rounded once.  Elements of X0 below 2^-38 count as zero (so does a gradient
+ * whose norm is that far below 1e-7).  G and out are rows x cols, CN_F32, CN_F16 or CN_BF16 each; out may be G.  A zero G
+ * gives zeros, one that is not finite NaNs. */
 size_t cn_orthogonalize_workspace_bytes(int64_t rows, int64_t cols);
 cn_status cn_orthogonalize(const void *G_device, int dtype, int64_t rows, int64_t cols, int64_t ldg, int steps,
                            void *out_device, int out_dtype, int64_t ldo, void *workspace_device,

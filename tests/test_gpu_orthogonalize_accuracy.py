@@ -51,6 +51,30 @@ def _gradient(torch, rows, cols, kind, gen):
     return G
 
 
+KINDS = ["one row", "two rows", "sixteen rows", "equal rows", "one column", "half of the rows", "one direction", "noise"]
+
+
+@pytest.mark.parametrize("rows,cols", [(140, 5000), (256, 6000), (700, 2900), (2900, 700), (100, 900), (300, 300)])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_few_rows_and_directions(torch, rows, cols, kind, dtype):
+    """Where few rows, columns or directions carry the gradient, roundings do not average out: their root mean square over
+    several gradients.  A number in two fp16 parts is off by up to 2^-23 of its power of two, one in fp32 by 2^-24: 1.15 and 0.58 times
+    2^-24, root mean square.  A product leaves out lo lo, two errors of up to 2^-11: 1.33 times 2^-24 where a sum has one term,
+    less where it has more.  A step rounds A, P and X and computes three products from them: sqrt(3 * 1.15^2 + 3 * 1.33^2)
+    against sqrt(3 * 0.58^2), so no more than 3.05 times as far as plain fp32."""
+    import clusternet_amd as cn
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    ours = plain = 0.0
+    for _ in range(6):
+        G = _gradient(torch, rows, cols, kind, gen).to(getattr(torch, dtype))
+        want = _steps(G.double())
+        far = lambda x: float((x.double() - want).norm() / want.norm()) ** 2 / 6  # noqa: E731
+        ours += far(cn.orthogonalize(G, out=torch.empty(rows, cols, device="cuda")))
+        plain += far(_steps(G.float()))
+    assert ours ** 0.5 <= 3.05 * plain ** 0.5, (ours ** 0.5, plain ** 0.5, (ours / plain) ** 0.5)
+
+
 @pytest.mark.parametrize("rows,cols", [(100, 333), (784, 1024), (2100, 2050), (3000, 700), (700, 2900)])
 @pytest.mark.parametrize("kind", ["noise", "strong"])
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
