@@ -767,12 +767,6 @@ static int stream_grid(const Context *ctx, size_t n, int per_cu) {
     return (int)(g < 1 ? 1 : g);
 }
 
-template <typename Kernel>
-static cn_status with_table_space(Kernel kernel, int bytes) {
-    CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    return CN_OK;
-}
-
 static cn_status compress_impl(const char *who, const float *x, float precision, const float *precision_dev, size_t n,
                                uint8_t *codes, float alpha, float *y, void *stream) {
     if (n == 0) return CN_OK;
@@ -784,24 +778,14 @@ static cn_status compress_impl(const char *who, const float *x, float precision,
     const int lds_all = (int)sizeof(EncodeShared) + 256 * (int)sizeof(float);  // with the update's decode table
     const int lds = (int)sizeof(EncodeShared) + (y ? 256 * (int)sizeof(float) : 0);
     static OncePerDevice configured;
-    if (configured.first(ctx->device)) {
-        cn_status c = CN_OK;
-        if (c == CN_OK) c = with_table_space(&compress_kernel<true, false, false>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_kernel<false, false, false>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_kernel<true, true, false>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_kernel<false, true, false>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_kernel<true, false, true>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_kernel<false, false, true>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_kernel<true, true, true>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_kernel<false, true, true>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_stream_kernel<1024, 12, false, false>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_stream_kernel<1024, 12, false, true>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_stream_kernel<512, 10, false, false>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_stream_kernel<512, 10, false, true>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_stream_kernel<1024, 4, true, false>, lds_all);
-        if (c == CN_OK) c = with_table_space(&compress_stream_kernel<1024, 4, true, true>, lds_all);
-        if (c != CN_OK) return c;
-    }
+    s = configured.lds(ctx->device, lds_all, &compress_kernel<true, false, false>, &compress_kernel<false, false, false>,
+                       &compress_kernel<true, true, false>, &compress_kernel<false, true, false>,
+                       &compress_kernel<true, false, true>, &compress_kernel<false, false, true>,
+                       &compress_kernel<true, true, true>, &compress_kernel<false, true, true>,
+                       &compress_stream_kernel<1024, 12, false, false>, &compress_stream_kernel<1024, 12, false, true>,
+                       &compress_stream_kernel<512, 10, false, false>, &compress_stream_kernel<512, 10, false, true>,
+                       &compress_stream_kernel<1024, 4, true, false>, &compress_stream_kernel<1024, 4, true, true>);
+    if (s != CN_OK) return s;
     const bool vec = aligned(x, 16) && aligned(codes, 4) && (!y || aligned(y, 16));
     const bool tuned = g_workgroups_per_cu != 0;  // the tuning hook keeps the tile kernel and its grid
     int encoder = g_encoder;

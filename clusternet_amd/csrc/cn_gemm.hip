@@ -1183,10 +1183,8 @@ static cn_status launch_tile(const GemmArgs &args, int device, hipStream_t st) {
     size_t lds = (size_t)(G::NST * (TM + TN) * G::BK + (B_KIND == B_CODES ? 256 : 0)) * sizeof(float);
     if (lds < NW * 32 * 36 * sizeof(float)) lds = NW * 32 * 36 * sizeof(float);
     static OncePerDevice configured;
-    if (configured.first(device)) {
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&gemm_kernel<A_KC, B_KIND, TN, TM, EPI>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    }
+    const cn_status status = configured.lds(device, (int)lds, &gemm_kernel<A_KC, B_KIND, TN, TM, EPI>);
+    if (status != CN_OK) return status;
     hipLaunchKernelGGL((gemm_kernel<A_KC, B_KIND, TN, TM, EPI>), dim3(args.units), dim3(NT), lds, st, args);
     CN_HIP(hipGetLastError());
     return CN_OK;
@@ -1205,10 +1203,8 @@ static cn_status launch_persistent_tile(const GemmArgs &args, int num_cu, int de
     using G = Geo<128, TN>;
     const size_t lds = (size_t)(2 * (128 + TN) * G::BK + 4) * sizeof(float);  // the stages and the ticket word
     static OncePerDevice configured;
-    if (configured.first(device)) {
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&gemm_persistent_kernel<A_KC, B_IS_KC, TN>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    }
+    const cn_status status = configured.lds(device, (int)lds, &gemm_persistent_kernel<A_KC, B_IS_KC, TN>);
+    if (status != CN_OK) return status;
     const uint32_t slots = (uint32_t)num_cu * 2u;
     hipLaunchKernelGGL((gemm_persistent_kernel<A_KC, B_IS_KC, TN>), dim3(args.units < slots ? args.units : slots), dim3(NT), lds, st, args);
     CN_HIP(hipGetLastError());

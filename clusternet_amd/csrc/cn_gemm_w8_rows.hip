@@ -212,12 +212,8 @@ cn_status gemm_w8_rows(int splits, int64_t M, int64_t N, int64_t K, const float 
     if (splits > 1) { g.out = (float *)workspace; g.out_ld = N; g.plane = M * N; }
     else            { g.out = C; g.out_ld = ldc; g.plane = 0; }
     static OncePerDevice configured;
-    if (configured.first(device)) {
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&gemm_w8_rows_kernel<1, 4, 8>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes(8)));
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&gemm_w8_rows_kernel<2, 4, 8>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes(8)));
-    }
+    const cn_status status = configured.lds(device, (int)lds_bytes(8), &gemm_w8_rows_kernel<1, 4, 8>, &gemm_w8_rows_kernel<2, 4, 8>);
+    if (status != CN_OK) return status;
     const dim3 grid((unsigned)(g.tiles_n * g.tiles_m * splits));
     if (M <= 32)      hipLaunchKernelGGL((gemm_w8_rows_kernel<1, 4, 8>), grid, dim3(512), lds_bytes(8), st, g);
     else              hipLaunchKernelGGL((gemm_w8_rows_kernel<2, 4, 8>), grid, dim3(512), lds_bytes(8), st, g);

@@ -5,6 +5,9 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <mutex>
+
 #include "../../include/cnhip.h"
 #include "../../include/cnhip_hooks.h"
 
@@ -67,14 +70,31 @@ constexpr int kTicketGroup = 8;
 constexpr int kTicketStride = 32;
 constexpr int kTicketWords = (1 + kReduceSlots / kTicketGroup) * kTicketStride;
 
-// A kernel's attributes (its dynamic LDS limit) are set per device: one flag per device for a call site.
+// A kernel's attributes (its dynamic LDS limit) are set per device: one object for a call site.  run(device, configure) returns
+// CN_OK once `configure` has succeeded there; a first call on another thread waits for it (its launch needs the attributes too),
+// and a failure is reported and tried again by the next call.
 struct OncePerDevice {
-    bool done[kMaxDevices] = {};
-    bool first(int device) {
-        if (device < 0 || device >= kMaxDevices) return true;
-        const bool was = done[device];
-        done[device] = true;
-        return !was;
+    std::atomic<bool> done[kMaxDevices] = {};
+    std::mutex mutex;
+    template <typename F>
+    cn_status run(int device, F &&configure) {
+        if (device < 0 || device >= kMaxDevices) return configure();
+        if (done[device].load(std::memory_order_acquire)) return CN_OK;
+        std::lock_guard<std::mutex> lock(mutex);
+        if (done[device].load(std::memory_order_relaxed)) return CN_OK;
+        const cn_status s = configure();
+        if (s == CN_OK) done[device].store(true, std::memory_order_release);
+        return s;
+    }
+    // The usual case: room for `bytes` of dynamic LDS for each of the kernels.
+    template <typename... K>
+    cn_status lds(int device, int bytes, K *...kernels) {
+        return run(device, [&]() -> cn_status {
+            hipError_t e = hipSuccess;
+            ((e = e == hipSuccess ? hipFuncSetAttribute(reinterpret_cast<const void *>(kernels), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : e), ...);
+            CN_HIP(e);
+            return CN_OK;
+        });
     }
 };
 

@@ -409,8 +409,8 @@ cn_status cn_transpose_f32(const float *in, int64_t rows, int64_t cols, float *o
     auto tiled = [&](auto kernel, int edge) -> cn_status {
         const int lds = edge * (edge + 1) * (int)sizeof(float);
         static OncePerDevice configured[2][2];
-        if (configured[edge == 128][vec].first(ctx->device))
-            CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        const cn_status status = configured[edge == 128][vec].lds(ctx->device, lds, kernel);
+        if (status != CN_OK) return status;
         const int64_t tiles_r = (rows + edge - 1) / edge, tiles = tiles_r * ((cols + edge - 1) / edge);
         hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(edge * edge / 16), lds, st, in, rows, cols, out, tiles_r);
         CN_HIP(hipGetLastError());
@@ -424,8 +424,8 @@ cn_status cn_transpose_f32(const float *in, int64_t rows, int64_t cols, float *o
         // 40000: 5.8 against 5.5; 8192 x 100096: 6.15 either way; 4096 x 4096: 31 us against 24, hence the bound)
         const int lds = 128 * 129 * (int)sizeof(float);
         static OncePerDevice drawn_configured;
-        if (drawn_configured.first(ctx->device))
-            CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&transpose_drawn_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        const cn_status status = drawn_configured.lds(ctx->device, lds, &transpose_drawn_kernel);
+        if (status != CN_OK) return status;
         hipLaunchKernelGGL(transpose_drawn_kernel, dim3(ctx->num_cu), dim3(1024), lds, st, in, rows, cols, out, (rows + 127) / 128,
                            (uint32_t)tiles128, counter);
         CN_HIP(hipGetLastError());

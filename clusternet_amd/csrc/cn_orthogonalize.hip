@@ -891,9 +891,8 @@ Space lay_out(void *workspace, const Sizes &z) {
 template <int TILE, int TERMS, int FINISH>
 cn_status run_product(const Product &g, const Cut &c, int device, hipStream_t st) {
     static OncePerDevice configured;
-    if (configured.first(device))
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&product_kernel<TILE, TERMS, FINISH>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                   lds_of<TILE>()));
+    const cn_status status = configured.lds(device, lds_of<TILE>(), &product_kernel<TILE, TERMS, FINISH>);
+    if (status != CN_OK) return status;
     hipLaunchKernelGGL((product_kernel<TILE, TERMS, FINISH>), dim3(c.workgroups), dim3(threads_of<TILE>()), lds_of<TILE>(), st, g);
     if (c.slots > 0)
         hipLaunchKernelGGL((join_kernel<TILE, FINISH>), dim3((c.tiles - c.whole) * (TILE / 32) * (TILE / 32) / 4), dim3(256), 0, st, g, c.whole);

@@ -4,7 +4,10 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <chrono>
 #include <mutex>
+#include <thread>
+#include <vector>
 
 #include "cn_internal.h"
 #include "cn_xlut.h"
@@ -202,6 +205,30 @@ const char *cn_status_string(cn_status s) {
 const char *cn_last_error(void) { return g_error; }
 
 void cn_host_reduction_fences(int enabled) { g_reduction_fences = enabled != 0; }
+
+// Test hook: `threads` threads configure a fresh OncePerDevice at once; the first `failures` attempts fail (pure host logic).
+void cn_host_once_per_device(int threads, int failures, int *attempts_out, int *failed_out, int *early_out) {
+    OncePerDevice once;
+    std::atomic<int> attempts{0}, failed{0}, early{0};
+    std::atomic<bool> configured{false};
+    std::vector<std::thread> all;
+    for (int i = 0; i < threads; ++i)
+        all.emplace_back([&] {
+            const cn_status s = once.run(0, [&]() -> cn_status {
+                const int attempt = attempts++;
+                std::this_thread::sleep_for(std::chrono::milliseconds(20));  // long enough for every thread to be here
+                if (attempt < failures) return CN_ERR_HIP;
+                configured = true;
+                return CN_OK;
+            });
+            if (s != CN_OK) ++failed;
+            else if (!configured) ++early;
+        });
+    for (std::thread &t : all) t.join();
+    *attempts_out = attempts;
+    *failed_out = failed;
+    *early_out = early;
+}
 
 // Test hook: after a device synchronisation, the number of ticket counters of the current device that are not zero
 // (kernels that draw their tiles leave theirs at zero), or -1 if the device is not initialised.

@@ -1165,10 +1165,8 @@ static cn_status csr_gemm(const char *who, int64_t R, int64_t Cc, int64_t N, con
     if (!out && g_lds_rows && Cc > 0 && Cc <= kLdsMaxRows) {  // maximum only, B strip in LDS
         const int lds_rows = (int)(Cc * kLdsStrip * sizeof(float));
         static OncePerDevice lds_configured;
-        if (lds_configured.first(ctx->device)) {
-            CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&csr_rows_max_lds_kernel),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMaxRows * kLdsStrip * (int)sizeof(float)));
-        }
+        s = lds_configured.lds(ctx->device, kLdsMaxRows * kLdsStrip * (int)sizeof(float), &csr_rows_max_lds_kernel);
+        if (s != CN_OK) return s;
         const int64_t strips = (N + kLdsStrip - 1) / kLdsStrip;
         if (strips > 0x7fffffLL) { set_error("%s: too many columns", who); return CN_ERR_SHAPE; }
         int64_t parts = (int64_t)ctx->num_cu / strips;  // one workgroup per compute unit
@@ -1303,21 +1301,10 @@ static cn_status csr_gemm_coded(const char *who, int64_t R, int64_t Cc, int64_t 
     hipStream_t st = (hipStream_t)stream;
     const int lds = (int)sizeof(EncodeShared) + 256 * (int)sizeof(float);
     const int lds_paired = lds + 2 * kProducers * kPatchWords * (int)sizeof(uint32_t);
-    static OncePerDevice configured;
-    if (configured.first(ctx->device)) {
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&csr_gemm_coded_kernel),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&csr_rows_kernel<2>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&csr_rows_kernel<3>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&csr_rows_kernel<4>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&csr_rows_kernel<5>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds_paired));
-        CN_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&csr_rows_kernel<6>),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds_paired));
-    }
+    static OncePerDevice configured, paired_configured;
+    s = configured.lds(ctx->device, lds, &csr_gemm_coded_kernel, &csr_rows_kernel<2>, &csr_rows_kernel<3>, &csr_rows_kernel<4>);
+    if (s == CN_OK) s = paired_configured.lds(ctx->device, lds_paired, &csr_rows_kernel<5>, &csr_rows_kernel<6>);
+    if (s != CN_OK) return s;
     const bool vec = Cc > 0 && Cc * ldb < (1LL << 30) && aligned(B, 16) && ldb % 4 == 0 && N % 4 == 0 && aligned(codes, 4) &&
                      (!w || (aligned(w, 16) && ldw % 4 == 0)) && (!rms || aligned(rms, 16));
     if (vec) {

@@ -75,6 +75,11 @@ int cn_host_tile_counters_in_use(void);
  * key -1 (its kernels then take the form that does not draw).  Pure host logic. */
 void cn_host_stream_slots(const uint64_t *keys, int n, int *slots_out);
 
+/* The library's per-device configuration of a call site, on a fresh instance: `threads` threads make their first call at once,
+ * the first `failures` attempts to configure fail.  *attempts_out: how often it was configured; *failed_out: calls that
+ * reported a failure; *early_out: calls that went on before anything was configured.  Pure host logic. */
+void cn_host_once_per_device(int threads, int failures, int *attempts_out, int *failed_out, int *early_out);
+
 /* cn_absmax_compress_8bit as one launch (abs-max, a wait across the resident grid, compression) instead of as two
  * kernels: 1 = wherever the single launch can run (aligned tensors below 2^26 elements), 0 = never, negative = the
  * library's own choice by size.  Same bits. */
