@@ -2,7 +2,10 @@
 // vocabulary of its window language model with one atomic per element (kConstructVocabMatrix, kUpdateVocabWithGradient,
 // source/clusterKernels.cu:1497-1712); here the gradient's sums run over sorted tokens, so they do not depend on scheduling.
 //
-// Lookup      out[t] = round(scale * E[tok[t]]).  Bound by memory: every row read once, every output written once.
+// Lookup      out[t] = round(scale * E[tok[t]]).  Bound by memory: every row read once, every output written once.  16 bytes an
+//             access where the width, both leading dimensions and both addresses are multiples of that; one element an access
+//             otherwise, which 16-bit rows feel most (65536 tokens: 120 fp32 columns 9.6 us, 121 17.5; 2048 bf16 columns 61, 2047
+//             327; the whole gradient of 2048 285, of 2047 795).
 //
 // Gradient    dE[v] = scale * sum over {t : tok[t] = v} of dY[t], in fp32.
 //   Up to kDirectItems positions and rows that are not wide: see grad_direct_kernel.  Otherwise:
@@ -396,8 +399,11 @@ __global__ __launch_bounds__(256) void grad_chunks_kernel(GradArgs a, const T *_
 // every per-th of them, and the groups' sums are added in order.  At most 32 lanes a row, so that per is 8 or more: even if all
 // positions name one row, no more than 256 are added one after the other, kDirectAhead in flight.  (128 windows of 11 words x
 // 120, fp32: 7.6 us, 19.9 by sorting; 2048 positions 8 and 21, all of them the same row 28.5 and 23.3.)  Every slab of
-// columns compares anew: two at most (four: 2048 x 1024 bf16 in 17 us, by sorting in 20, all the same row in 65 and 25).  Rows of
-// up to 256 elements always go this way, so that such calls need no workspace; wider ones where 16 bytes a lane cover them in two.
+// columns compares anew: two at most where 16 bytes a lane are taken (four: 2048 x 1024 bf16 in 17 us, by sorting in 20, all the
+// same row in 65 and 25).  Rows of up to 256 elements always go this way, so that such calls need no workspace, even where they are
+// not made of whole vectors and a lane takes one element: up to eight slabs then (2048 x 65 fp32 12 us, all the same row 31;
+// x 129 17 and 34; x 255 24 and 39, where 257 columns are sorted in 20 and 24: a few microseconds at the far end, not worth a
+// second contract for the workspace).  Wider rows go this way where 16 bytes a lane cover them in two slabs.
 constexpr int kDirectItems = 2048, kDirectLanes = 32, kDirectSlabs = 2, kDirectAhead = 8;
 
 template <typename T, typename E, typename I, int VEC>

@@ -38,7 +38,7 @@
 // computes a whole tile applies the formula to its accumulators and writes the next operand in both orientations; parts of a
 // tile go to memory and a second kernel adds them in order.  Either way the result does not depend on scheduling.
 //
-// Measured (one MI355X): X^T Q of 4096 x 16384 in 1.34 ms, 1.23 PFLOP/s of fp16 products with the write-out of X and X^T in it
+// Measured (one MI355X): X^T P of 4096 x 16384 in 1.38 ms, 1.20 PFLOP/s of fp16 products with the write-out of X and X^T in it
 // (0.8 GB, of which little overlaps); the library's own 8192^3 fp16 product reaches 1.31 on the same card.  The chip runs
 // at its power limit (1.75 GHz on random numbers, 2.1 on zeros), so what would be won by fewer stalls is lost in clock.
 #include "cn_dtypes.h"

@@ -57,7 +57,8 @@ struct GemmW4Args {
     void *out;
     int64_t M, N, K, lda, ldo;
     int tiles_k, tiles_n;
-    int vec_a;             // rows of A allow 16-byte loads
+    int vec_a;             // rows of A allow 16-byte loads; others go element by element, with nothing requested ahead (1 x 5000 x 16384
+                           // bf16 12.7 us, 4999 24.0; 13 x 5000 x 1999 fp32 12.0, 5001 27.5; 64 x 8192 x 16384 bf16 51, 8191 154)
 };
 
 // A operand of one instruction as the words of its kind, and how many of them a number needs.
