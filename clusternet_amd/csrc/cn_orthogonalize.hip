@@ -11,21 +11,22 @@
 // above the diagonal are computed).  In fp32 the matrix cores give 157 TFLOP/s; here each operand is kept as two fp16
 // numbers, x 2^14 = hi + lo (2^10 for P), and a product is the three fp16 products hi hi + hi lo + lo hi in fp32
 // accumulators.  What is left out, lo lo, and the rounding of lo are 2^-22 of the product, so the result is about as far from
-// the exact one as plain fp32 products leave it.  Root mean square over gradients, twelve sizes from 16 x 3000 to 4096 x 4096: 0.2 to
-// 1.4 times as far for Gaussian numbers, half of the rows zero, few strong directions; up to 2.4 times (and 1.2 10^-6 of
-// |out|) for gradients of one or two rows or of one column, where roundings do not average out.  The factors keep entries
-// below 65504 (|X| <= 1.21, |A| <= 1.46, |P| <= 2.81) and lo above the smallest fp16 number for entries down to 2^-13 of
+// the exact one as plain fp32 products leave it.  Root mean square over gradients, five steps, 16 x 3000, 64 x 64, 64 x 16384,
+// 140 x 5000, 256 x 6000, 300 x 300, 700 x 2900, 784 x 1024, 1000 x 4001, 2048 x 2048 and 4096 x 4096: 0.2 to 1.4 times as far for
+// Gaussian numbers, half of the rows zero, few strong directions; up to 2.4 times (and 1.2 10^-6 of |out|) for gradients
+// of one or two rows or of one column, where roundings do not average out.  The factors keep entries below 65504 (|X| <=
+// 1.21, |A| <= 1.46, |P| <= 2.81) and lo above the smallest fp16 number for entries down to 2^-13 of
 // the largest.  a X stays outside the product, with X read back as hi + lo: folding a into P's diagonal costs a factor of
 // three in accuracy for nearly low-rank gradients.
 //
 // Several steps on m x m matrices alone, with X updated once at their end (A and its polynomials commute; 6.6 ms in place of
 // 10.8 for 4096 x 16384), are not sound in these numbers: the polynomial Q of two or three steps has entries of up to 12 or 41 where a
-// row has a large singular value to itself, and (a^g + Q) X, of about 1, keeps their rounding: 4 10^-6 to 10^-5 of |out| for
-// gradients of one or two rows or of one column, up to twenty times plain fp32.
+// row has a large singular value to itself, and (a^g + Q) X, of about 1, keeps their rounding: 4 10^-6 to 9 10^-6 of |out| for
+// gradients of one or two rows or of one column, up to 11 times plain fp32.
 //
 // A gradient of 16 bits is its own hi if only the power of two of the scale is applied to it, so X0 X0^T is one product and P X0
-// two, with nothing lost; the rest of the scale, in [1, 2), goes to their results (split_kernel).  (One product in place of
-// three in later steps too is not sound: hi alone is off by up to 2^-11 the same way in all equal entries, such as the
+// two, with nothing lost but the rounding of the rest of the scale, in [1, 2), which goes to their results (split_kernel).
+// (One product in place of three in later steps too is not sound: hi alone is off by up to 2^-11 the same way in all equal entries, such as the
 // diagonal of A for orthogonal rows, and the next steps multiply that by ten: 5 10^-3 of |out| for 17 x 498.)
 //
 // Layout: a matrix is blocks of 256 rows, in them groups of 32 columns: a 128-byte line per row, 32 hi, then 32 lo.  A stage of

@@ -22,8 +22,8 @@
 //     maxout and sigmoid outputs, rows near 1), where they were up to 35 times those.
 //   * Where a may be as large as fp32 goes, the operands are 2^-13 (16 + q), 2^-13 in place of 1, and 2^-11 (q - z) (another
 //     exponent in the same pattern): 128 of the largest fit fp32, where same-signed rows from 8 10^34 on would overflow.
-//     The factor comes back in the write-out: all sums keep 2^-136, half a step of the smallest normal bf16 number.  (Given
-//     to the scales, which then need a place for those above 2^115: 5 % for groups of 32.)
+//     The factor comes back in the write-out: all sums keep 2^-136, less than half a step of the smallest normal bf16
+//     number.  (Given to the scales, which then need a place for those above 2^115: 5 % for groups of 32.)
 //   * Products are exact: a 16-bit a times a whole number up to 31 fits fp32; a of fp32 enters as three bf16 numbers that add
 //     up to it exactly (8 bits of it each).  The sums, the scales and everything behind them are fp32; a 16-bit result is
 //     rounded once.

@@ -77,3 +77,18 @@ def test_large_and_small_scales_and_rows(torch, dtype, group, zero_points, size,
     a = torch.from_numpy((rows * rng.uniform(-1, 1, (5, 200))).astype(np.float32)).cuda().to(getattr(torch, dtype))
     if bool(a.isfinite().all()):  # (fp16 holds no 1e30)
         _holds(torch, a, w4)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("group,zero_points", [(32, True), (64, False), (128, False)])
+@pytest.mark.parametrize("M", [4, 20])
+def test_rows_that_are_not_finite(torch, dtype, group, zero_points, M):
+    """NaN all along them, whatever the weights, and nothing of it in other rows."""
+    import clusternet_amd as cn
+    w4 = _weights(torch, 200, 40, group, zero_points, 0.1)
+    a = torch.randn(M, 200, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).to(getattr(torch, dtype))
+    want = cn.gemm_w4(a, w4)
+    a[1, 0], a[2, 199], a[3, 64] = float("nan"), float("inf"), -float("inf")
+    out = cn.gemm_w4(a, w4)
+    rest = [0, *range(4, M)]
+    assert bool(out[1:4].isnan().all()) and torch.equal(out[rest], want[rest])
